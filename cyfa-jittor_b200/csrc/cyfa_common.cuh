@@ -29,6 +29,7 @@ enum DeviceError : int {
   kErrNone = 0,
   kErrWaitTimeout = 1,
   kErrBadShape = 2,
+  kErrBadIndex = 3,  // a token outside the vocabulary
 };
 
 __device__ __forceinline__ void set_error(int code) { atomicCAS(&g_device_error, 0, code); }

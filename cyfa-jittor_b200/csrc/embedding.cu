@@ -1,0 +1,413 @@
+// Embedding lookup with a scale, and the gradient of the whole table.
+//   out[n] = scale W[id_n]
+//   dW[v]  = scale sum over {n : id_n = v} of dout[n], in ascending n, fp32
+// The sum runs over the tokens sorted by id (a stable radix sort, so equal ids
+// keep their order): no float atomics, the same bits on every run.  A token
+// outside the vocabulary sets the device error word, reads as a zero row and
+// has no gradient; the padding row's gradient is zero.
+#include <algorithm>
+#include <type_traits>
+
+#include "cyfa_common.cuh"
+
+namespace cyfa {
+
+constexpr int kEmbThreads = 256;
+
+// VEC elements per access; the widest that divides D and fits the pointers.
+template <typename T, int VEC>
+struct EmbVec {
+  typedef typename std::conditional<
+      sizeof(T) * VEC == 16, uint4,
+      typename std::conditional<
+          sizeof(T) * VEC == 8, uint2,
+          typename std::conditional<sizeof(T) * VEC == 4, uint32_t, uint16_t>::type>::type>::type U;
+  static __device__ __forceinline__ void load(const T* p, float* f) {
+    const U u = *reinterpret_cast<const U*>(p);
+    const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = float(e[i]);
+  }
+  static __device__ __forceinline__ void store(T* p, const float* f) {
+    U u;
+    T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) e[i] = T(f[i]);
+    *reinterpret_cast<U*>(p) = u;
+  }
+};
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kEmbThreads)
+    embed_fwd_kernel(const long long* tokens, const T* w, T* out, long long N, long long V, int D,
+                     float scale) {
+  pdl_wait();
+  pdl_trigger();
+  const int per_row = D / VEC;
+  const long long total = N * per_row;
+  for (long long i = (long long)blockIdx.x * kEmbThreads + threadIdx.x; i < total;
+       i += (long long)gridDim.x * kEmbThreads) {
+    const long long n = i / per_row;
+    const int c = int(i - n * per_row) * VEC;
+    const long long id = tokens[n];
+    float f[VEC];
+    if (id >= 0 && id < V) {
+      EmbVec<T, VEC>::load(w + id * D + c, f);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) f[k] *= scale;
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) f[k] = 0.f;
+      if (c == 0) set_error(kErrBadIndex);
+    }
+    EmbVec<T, VEC>::store(out + n * D + c, f);
+  }
+}
+
+// ------------------------------------------------------------------- the sort
+// Stable radix sort of (id, position), 8 bits a pass.  A CTA takes kSortTile
+// consecutive entries, each of its warps a run of them; ranks inside a run come
+// from match masks, across runs and tiles from counts per digit.
+constexpr int kSortThreads = 256;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortRounds = 16;  // entries of a lane
+constexpr int kSortTile = kSortThreads * kSortRounds;
+
+__device__ __forceinline__ uint32_t sort_key(const long long* tokens, long long V, long long pad,
+                                             long long n) {
+  const long long id = tokens[n];
+  return id >= 0 && id < V && id != pad ? uint32_t(id) : uint32_t(V);  // dropped ids come last
+}
+
+// first pass: keys from the tokens, positions from the index
+struct SortPass {
+  const long long* tokens;  // first pass, else null
+  const uint32_t* key_in;
+  const uint32_t* pos_in;
+  uint32_t* key_out;
+  uint32_t* pos_out;
+  uint32_t* count;  // [256][tiles]
+  long long N, V, pad;
+  int shift, tiles;
+};
+
+__device__ __forceinline__ uint32_t pass_key(const SortPass& p, long long n) {
+  return p.tokens ? sort_key(p.tokens, p.V, p.pad, n) : p.key_in[n];
+}
+
+__global__ void __launch_bounds__(kSortThreads) embed_sort_count_kernel(SortPass p) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ uint32_t hist[256];
+  hist[threadIdx.x] = 0;
+  __syncthreads();
+  const long long n0 = (long long)blockIdx.x * kSortTile;
+  for (int i = threadIdx.x; i < kSortTile; i += kSortThreads)
+    if (n0 + i < p.N) atomicAdd(&hist[(pass_key(p, n0 + i) >> p.shift) & 255], 1u);
+  __syncthreads();
+  p.count[(size_t)threadIdx.x * p.tiles + blockIdx.x] = hist[threadIdx.x];
+}
+
+// exclusive scan of count[256 * tiles], one CTA
+__global__ void __launch_bounds__(1024) embed_sort_scan_kernel(uint32_t* count, int n) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ uint32_t part[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (n + 1023) / 1024, b = min(n, tid * per), e = min(n, b + per);
+  uint32_t sum = 0;
+  for (int i = b; i < e; ++i) sum += count[i];
+  uint32_t inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 31) part[warp] = inc;
+  __syncthreads();
+  uint32_t before = inc - sum;
+  for (int w = 0; w < warp; ++w) before += part[w];
+  for (int i = b; i < e; ++i) {
+    const uint32_t v = count[i];
+    count[i] = before;
+    before += v;
+  }
+}
+
+__global__ void __launch_bounds__(kSortThreads) embed_sort_move_kernel(SortPass p) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ uint32_t next[kSortWarps][256];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int i = tid; i < kSortWarps * 256; i += kSortThreads) (&next[0][0])[i] = 0;
+  __syncthreads();
+  const long long n0 = (long long)blockIdx.x * kSortTile + warp * (32 * kSortRounds);
+  uint32_t key[kSortRounds];
+#pragma unroll
+  for (int r = 0; r < kSortRounds; ++r) {
+    const long long n = n0 + r * 32 + lane;
+    const bool in = n < p.N;
+    key[r] = in ? pass_key(p, n) : 0u;
+    const unsigned same =
+        __match_any_sync(0xffffffffu, in ? (key[r] >> p.shift) & 255u : 256u);
+    if (in && lane == __ffs(same) - 1) next[warp][(key[r] >> p.shift) & 255] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  {
+    uint32_t run = p.count[(size_t)tid * p.tiles + blockIdx.x];
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) {
+      const uint32_t c = next[w][tid];
+      next[w][tid] = run;
+      run += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kSortRounds; ++r) {
+    const long long n = n0 + r * 32 + lane;
+    const bool in = n < p.N;
+    const uint32_t d = (key[r] >> p.shift) & 255u;
+    const unsigned same = __match_any_sync(0xffffffffu, in ? d : 256u);
+    if (in) {
+      const uint32_t at = next[warp][d] + __popc(same & ((1u << lane) - 1));
+      p.key_out[at] = key[r];
+      p.pos_out[at] = p.pos_in ? p.pos_in[n] : uint32_t(n);
+    }
+    __syncwarp();
+    if (in && lane == __ffs(same) - 1) next[warp][d] += __popc(same);
+    __syncwarp();
+  }
+}
+
+// ------------------------------------------------------------------- the sums
+// The sorted entries in pieces of kPiece: CTA (piece, columns) adds the rows of
+// each run of equal ids.  A run inside the piece is written at once.  A run that
+// began in an earlier piece leaves its part in head[piece], one that goes on
+// into the next leaves the part from its beginning in tail[piece]; those parts
+// are joined in order by embed_join_kernel.
+constexpr int kPiece = 32;
+constexpr int kSumThreads = 128;
+
+struct EmbSumParams {
+  const uint32_t* key;
+  const uint32_t* pos;
+  const void* dout;  // [N, D]
+  void* dw;          // [V, D], zeroed
+  float* head;       // [pieces, D]
+  float* tail;       // [pieces, D]
+  long long N;
+  uint32_t V;
+  int D;
+  float scale;
+};
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kSumThreads) embed_sum_kernel(EmbSumParams p) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ uint32_t key[kPiece + 2], pos[kPiece];  // key[0]: the entry before, key[cnt + 1]: after
+  const long long e0 = (long long)blockIdx.x * kPiece;
+  const int cnt = int(min((long long)kPiece, p.N - e0));
+  for (int i = threadIdx.x; i < cnt + 2; i += kSumThreads) {
+    const long long e = e0 + i - 1;
+    key[i] = e >= 0 && e < p.N ? p.key[e] : 0xffffffffu;
+    if (i >= 1 && i <= cnt) pos[i - 1] = p.pos[e];
+  }
+  __syncthreads();
+  const int c = (blockIdx.y * kSumThreads + threadIdx.x) * VEC;
+  if (c >= p.D) return;
+  const T* src = static_cast<const T*>(p.dout) + c;
+  float acc[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+  bool opened = key[0] == key[1];  // the current run began in an earlier piece
+#pragma unroll 4
+  for (int i = 0; i < cnt; ++i) {
+    const uint32_t v = key[i + 1];
+    if (v >= p.V) break;  // the dropped entries: nothing after them counts
+    float f[VEC];
+    EmbVec<T, VEC>::load(src + (size_t)pos[i] * p.D, f);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] += f[k];
+    if (key[i + 2] == v && i + 1 < cnt) continue;
+    const bool goes_on = key[i + 2] == v;
+    if (opened || goes_on) {
+      float* d = (opened ? p.head : p.tail) + (size_t)blockIdx.x * p.D + c;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) d[k] = acc[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] *= p.scale;
+      EmbVec<T, VEC>::store(static_cast<T*>(p.dw) + (size_t)v * p.D + c, acc);
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+    opened = false;
+  }
+}
+
+// CTA (piece, columns): if a run begins in the piece and goes on, the run's
+// parts in order: tail[piece], then head of the pieces up to its end.
+template <typename T>
+__global__ void __launch_bounds__(256) embed_join_kernel(EmbSumParams p) {
+  pdl_wait();
+  pdl_trigger();
+  const long long b = blockIdx.x;
+  const long long last = b * kPiece + kPiece - 1;  // the piece's last entry
+  if (last + 1 >= p.N) return;
+  const uint32_t v = p.key[last];
+  if (v >= p.V || p.key[last + 1] != v) return;
+  if (b > 0 && p.key[b * kPiece] == v && p.key[b * kPiece - 1] == v) return;  // began earlier
+  long long lo = last + 1, hi = p.N - 1;  // last entry of the run
+  while (lo < hi) {
+    const long long mid = (lo + hi + 1) >> 1;
+    if (p.key[mid] <= v) lo = mid; else hi = mid - 1;
+  }
+  const long long end = lo / kPiece;
+  const int c = blockIdx.y * 256 + threadIdx.x;
+  if (c >= p.D) return;
+  float acc = p.tail[(size_t)b * p.D + c];
+  for (long long q = b + 1; q <= end; ++q) acc += p.head[(size_t)q * p.D + c];
+  static_cast<T*>(p.dw)[(size_t)v * p.D + c] = T(acc * p.scale);
+}
+
+static size_t embed_align(size_t n) { return (n + 255) / 256 * 256; }
+
+struct EmbWork {
+  uint32_t *key[2], *pos[2], *count;
+  float *head, *tail;
+  size_t bytes;
+  EmbWork(void* base, long long N, int D) {
+    const size_t tiles = size_t((N + kSortTile - 1) / kSortTile);
+    const size_t pieces = size_t((N + kPiece - 1) / kPiece);
+    size_t at = 0;
+    auto take = [&](size_t n) {
+      char* q = static_cast<char*>(base) + at;
+      at += embed_align(n);
+      return q;
+    };
+    for (int i = 0; i < 2; ++i) {
+      key[i] = reinterpret_cast<uint32_t*>(take(size_t(N) * 4));
+      pos[i] = reinterpret_cast<uint32_t*>(take(size_t(N) * 4));
+    }
+    count = reinterpret_cast<uint32_t*>(take(tiles * 256 * 4));
+    head = reinterpret_cast<float*>(take(pieces * D * 4));
+    tail = reinterpret_cast<float*>(take(pieces * D * 4));
+    bytes = at;
+  }
+};
+
+static int embed_vec(int D, int es, const void* a, const void* b) {
+  int vec = 16 / es;
+  while (vec > 1 && (D % vec || !aligned(a, size_t(vec) * es) || !aligned(b, size_t(vec) * es)))
+    vec /= 2;
+  return vec;
+}
+
+static int embed_checks(int dtype, long long N, long long V, int D) {
+  CYFA_REQUIRE(N > 0 && N < (1ll << 31) && V > 0 && V < (1ll << 31) && D > 0, kBadShape);
+  CYFA_REQUIRE(dtype == 0 || dtype == 1, kBadDtype);
+  return kOk;
+}
+
+}  // namespace cyfa
+
+extern "C" {
+
+int cyfa_embed_fwd(const long long* tokens, const void* weight, int dtype, void* out, long long N,
+                   long long V, int D, float scale, void* stream) {
+  CYFA_REQUIRE(tokens && weight && out, kNullPointer);
+  const int rc = embed_checks(dtype, N, V, D);
+  if (rc) return rc;
+  const int es = dtype == 1 ? 2 : 4;
+  CYFA_REQUIRE(aligned(tokens, 8) && aligned(weight, es) && aligned(out, es), kMisaligned);
+  const int vec = embed_vec(D, es, weight, out);
+  const long long n = N * (D / vec);
+  const unsigned grid = unsigned(std::min<long long>((n + kEmbThreads - 1) / kEmbThreads, 148 * 64));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+#define CYFA_EMB(T, VEC)                                                                       \
+  CYFA_LAUNCH("embed_fwd", s,                                                                  \
+              (launch_k(embed_fwd_kernel<T, VEC>, grid, kEmbThreads, 0, s, tokens,             \
+                        static_cast<const T*>(weight), static_cast<T*>(out), N, V, D, scale)))
+  if (dtype == 1) {
+    if (vec == 8) CYFA_EMB(__nv_bfloat16, 8);
+    else if (vec == 4) CYFA_EMB(__nv_bfloat16, 4);
+    else if (vec == 2) CYFA_EMB(__nv_bfloat16, 2);
+    else CYFA_EMB(__nv_bfloat16, 1);
+  } else {
+    if (vec == 4) CYFA_EMB(float, 4);
+    else if (vec == 2) CYFA_EMB(float, 2);
+    else CYFA_EMB(float, 1);
+  }
+#undef CYFA_EMB
+  return launch_status();
+}
+
+size_t cyfa_embed_bwd_work_bytes(long long N, int D) {
+  return N > 0 && D > 0 ? EmbWork(nullptr, N, D).bytes : 0;
+}
+
+int cyfa_embed_bwd(const long long* tokens, const void* dout, int dtype, void* dweight, long long N,
+                   long long V, int D, float scale, long long padding_idx, void* work,
+                   size_t work_bytes, void* stream) {
+  CYFA_REQUIRE(tokens && dout && dweight && work, kNullPointer);
+  const int rc = embed_checks(dtype, N, V, D);
+  if (rc) return rc;
+  const int es = dtype == 1 ? 2 : 4;
+  CYFA_REQUIRE(aligned(tokens, 8) && aligned(dout, es) && aligned(dweight, es) && aligned(work, 256),
+               kMisaligned);
+  const EmbWork w(work, N, D);
+  CYFA_REQUIRE(work_bytes >= w.bytes, kWorkspace);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = cudaMemsetAsync(dweight, 0, size_t(V) * D * es, s);
+  if (e != cudaSuccess) return -static_cast<int>(e);
+  SortPass p{tokens, nullptr, nullptr, w.key[0], w.pos[0], w.count, N, V, padding_idx, 0,
+             int((N + kSortTile - 1) / kSortTile)};
+  int cur = 0;
+  for (int shift = 0; shift < 32 && (V >> shift) > 0; shift += 8) {
+    p.shift = shift;
+    CYFA_LAUNCH("embed_sort_count", s,
+                (launch_k(embed_sort_count_kernel, unsigned(p.tiles), kSortThreads, 0, s, p)));
+    CYFA_LAUNCH("embed_sort_scan", s,
+                (launch_k(embed_sort_scan_kernel, 1, 1024, 0, s, w.count, p.tiles * 256)));
+    CYFA_LAUNCH("embed_sort_move", s,
+                (launch_k(embed_sort_move_kernel, unsigned(p.tiles), kSortThreads, 0, s, p)));
+    cur = p.key_out == w.key[0] ? 0 : 1;
+    p.tokens = nullptr;
+    p.key_in = w.key[cur];
+    p.pos_in = w.pos[cur];
+    p.key_out = w.key[1 - cur];
+    p.pos_out = w.pos[1 - cur];
+  }
+  EmbSumParams q{w.key[cur], w.pos[cur], dout, dweight, w.head, w.tail, N, uint32_t(V), D, scale};
+  const int vec = embed_vec(D, es, dout, dweight);
+  const unsigned pieces = unsigned((N + kPiece - 1) / kPiece);
+  const int cols = kSumThreads * vec;
+  CYFA_REQUIRE((D + cols - 1) / cols <= 65535, kBadShape);
+  const dim3 grid(pieces, unsigned((D + cols - 1) / cols));
+#define CYFA_EMB(T, VEC) \
+  CYFA_LAUNCH("embed_sum", s, (launch_k(embed_sum_kernel<T, VEC>, grid, kSumThreads, 0, s, q)))
+  if (dtype == 1) {
+    if (vec == 8) CYFA_EMB(__nv_bfloat16, 8);
+    else if (vec == 4) CYFA_EMB(__nv_bfloat16, 4);
+    else if (vec == 2) CYFA_EMB(__nv_bfloat16, 2);
+    else CYFA_EMB(__nv_bfloat16, 1);
+  } else {
+    if (vec == 4) CYFA_EMB(float, 4);
+    else if (vec == 2) CYFA_EMB(float, 2);
+    else CYFA_EMB(float, 1);
+  }
+#undef CYFA_EMB
+  if (pieces > 1) {
+    const dim3 jgrid(pieces - 1, unsigned((D + 255) / 256));
+    if (dtype == 1)
+      CYFA_LAUNCH("embed_join", s, (launch_k(embed_join_kernel<__nv_bfloat16>, jgrid, 256, 0, s, q)));
+    else
+      CYFA_LAUNCH("embed_join", s, (launch_k(embed_join_kernel<float>, jgrid, 256, 0, s, q)));
+  }
+  return launch_status();
+}
+
+}  // extern "C"

@@ -19,6 +19,7 @@ LIB_PATH = os.environ.get("CYFA_LIB") or os.path.join(_HERE, "libcyfa.so")
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
+_ll = ctypes.c_longlong
 
 # name -> argtypes (restype is int for all)
 _SIGNATURES = {
@@ -58,6 +59,13 @@ _SIGNATURES = {
     "cyfa_add_rmsnorm": [_vp, _vp, _vp, _f, _vp, _i, _i, _vp],
     "cyfa_decode_conv": [_vp, ctypes.c_longlong] + [_vp] * 9 + [_i] * 5 + [_vp],
     "cyfa_swiglu": [_vp, _vp, _i, _i, _vp],
+    "cyfa_token_logprobs_fwd": [_vp, _i] + [_ll] * 4 + [_i, _vp, _ll, _i] + [_vp] * 6,
+    "cyfa_token_logprobs_bwd": [_vp, _i] + [_ll] * 4 + [_i, _vp, _ll] + [_vp] * 6,
+    "cyfa_embed_fwd": [_vp, _vp, _i, _vp, _ll, _ll, _i, _f, _vp],
+    "cyfa_embed_bwd": [_vp, _vp, _i, _vp, _ll, _ll, _i, _f, _ll, _vp, ctypes.c_size_t, _vp],
+    "cyfa_residual_norm_fwd": [_vp] * 6,
+    "cyfa_residual_norm_bwd": [_vp] * 12 + [ctypes.c_size_t, _vp],
+    "cyfa_newton_schulz": [_vp] + [_i] * 5 + [_f] * 4 + [_vp, _vp, ctypes.c_size_t, _vp],
 }
 
 # size queries (restype size_t)
@@ -69,6 +77,9 @@ _SIZE_QUERIES = {
     "cyfa_gated_norm_work_bytes": [_i] * 2,
     "cyfa_gated_norm_bias_work_bytes": [_i] * 3,
     "cyfa_grad_clip_work_bytes": [],
+    "cyfa_embed_bwd_work_bytes": [_ll, _i],
+    "cyfa_residual_norm_bwd_work_bytes": [_ll, _i],
+    "cyfa_newton_schulz_work_bytes": [_i] * 3,
 }
 
 
@@ -83,6 +94,16 @@ class DecodeLayerArgs(ctypes.Structure):
                             "hk_out", "hv_out", "clock_out", "gate", "gate_bias",
                             "o_norm_weight", "y")] + \
         [(n, _f) for n in ("q_eps", "k_eps", "scale", "o_eps", "o_scale")]
+
+
+class ResidualNormArgs(ctypes.Structure):
+    """cyfa_residual_norm_args."""
+
+    _fields_ = [("rows", _ll), ("D", _i), ("dtype", _i)] + \
+        [(n, _vp) for n in ("x", "y", "gate")] + \
+        [(n, _ll) for n in ("x_stride", "y_stride", "gate_stride")] + \
+        [(n, _vp) for n in ("weight", "post_weight", "scale_vector")] + \
+        [("scale", _f), ("eps", _f)]
 
 
 class BucketPiece(ctypes.Structure):
@@ -186,7 +207,8 @@ def require_cuda(*tensors):
 
 
 def device_error(reset=True):
-    """Returns the device error word (1 = a bounded wait timed out)."""
+    """Returns the device error word (1 = a bounded wait timed out, 3 = a token
+    outside the vocabulary)."""
     return lib().cyfa_device_error(1 if reset else 0)
 
 

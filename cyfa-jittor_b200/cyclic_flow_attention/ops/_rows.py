@@ -1,0 +1,65 @@
+"""Argument helpers of the row-wise operators: dtype codes, the device guard and
+the mapping of a strided tensor's leading dimensions to rows."""
+
+import contextlib
+
+import torch
+
+from .. import _lib
+
+_NO_GUARD = contextlib.nullcontext()
+_CODES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def dtype_code(name, t):
+    code = _CODES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be float32 or bfloat16, got {t.dtype}")
+    return code
+
+
+def same_device(**tensors):
+    """Raises unless all tensors are CUDA tensors of one device."""
+    _lib.require_cuda(*tensors.values())
+    devices = {n: t.device for n, t in tensors.items() if t is not None}
+    if len(set(devices.values())) > 1:
+        raise ValueError("tensors must be on one device, got "
+                         + ", ".join(f"{n} on {d}" for n, d in devices.items()))
+
+
+def on_device(t):
+    """Makes t's device the current one (the library launches on the current
+    device and on its current stream)."""
+    if t.device.index == torch.cuda.current_device():
+        return _NO_GUARD
+    return torch.cuda.device(t.device)
+
+
+def row_levels(x, most):
+    """The leading dimensions of x as at most `most` (size, stride) levels,
+    outermost first, when its last dimension is dense; None if they need more."""
+    if x.shape[-1] > 1 and x.stride(-1) != 1:
+        return None
+    levels = []
+    for size, stride in zip(x.shape[:-1], x.stride()[:-1]):
+        if size == 1:
+            continue
+        if levels and levels[-1][1] == size * stride:
+            levels[-1] = (levels[-1][0] * size, stride)
+        else:
+            levels.append((size, stride))
+    return levels if len(levels) <= most else None
+
+
+def as_rows(x):
+    """(x, row stride) with x's leading dimensions one evenly spaced run of rows;
+    x is copied if they are not."""
+    levels = row_levels(x, 1)
+    if levels is None:
+        x = x.contiguous()
+        levels = row_levels(x, 1)
+    return x, (levels[0][1] if levels else x.shape[-1])
+
+
+def f32(t):
+    return None if t is None else t.detach().to(torch.float32).contiguous()

@@ -1,0 +1,153 @@
+"""A block's residual add with the norms on both sides of it, with gradients.
+
+The reference writes it as separate framework ops (residual = x + y and RMSNorm,
+models/cyfa/modeling_cyfa.py:52-55,64-69; RMSNorm layers/cyfa.py:62-135); here the
+add, the branch's gate and scale, and both norms are one libcyfa launch forward
+and one, plus the parameter sums, backward.
+"""
+
+import ctypes
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+from ._rows import as_rows, dtype_code, f32, on_device, same_device
+
+MAX_WIDTH = 8192
+
+
+def _args(x, y, gate, weight, post, scale_vector, scale, eps):
+    """The call's argument block and the tensors that have to outlive it."""
+    D = x.shape[-1]
+    x, sx = as_rows(x)
+    sy = sg = 0
+    if y is not None:
+        y, sy = as_rows(y)
+    if gate is not None:
+        gate, sg = as_rows(gate)
+    p = lambda t: None if t is None else t.data_ptr()
+    return _lib.ResidualNormArgs(
+        x.numel() // D, D, dtype_code("x", x), p(x), p(y), p(gate), sx, sy, sg, p(weight),
+        p(post), p(scale_vector), scale, eps), (x, y, gate)
+
+
+def _forward(x, y, weight, post, gate, scale_vector, scale, eps):
+    """(xn or None, h, rstd_x, rstd_y)."""
+    rows = x.numel() // x.shape[-1]
+    dev = x.device
+    xn = None if y is None else torch.empty(x.shape, device=dev, dtype=x.dtype)
+    h = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    rstd = torch.empty(2 if post is not None else 1, rows, device=dev, dtype=torch.float32)
+    rstd_x = rstd[0]
+    rstd_y = rstd[1] if post is not None else None
+    if rows:
+        args, _keep = _args(x, y, gate, weight, post, scale_vector, scale, eps)
+        with on_device(x):
+            _lib.call("cyfa_residual_norm_fwd", ctypes.byref(args), _lib.ptr(xn), h.data_ptr(),
+                      rstd_x.data_ptr(), _lib.ptr(rstd_y), _lib.stream())
+    return xn, h, rstd_x, rstd_y
+
+
+class ResidualNormFunction(torch.autograd.Function):
+    """Autograd wrapper over cyfa_residual_norm_fwd / _bwd."""
+
+    @staticmethod
+    def forward(ctx, x, y, weight, post, gate, scale_vector, scale, eps):
+        ctx.set_materialize_grads(False)
+        w, pw, sv = f32(weight), f32(post), f32(scale_vector)
+        xn, h, rstd_x, rstd_y = _forward(x, y, w, pw, gate, sv, scale, eps)
+        plain = post is None and gate is None and scale_vector is None and scale == 1.0
+        # the plain sum needs y for no gradient
+        ctx.save_for_backward(x if xn is None else xn, None if plain else y, w, pw, gate, sv,
+                              rstd_x, rstd_y)
+        ctx.meta = (scale, eps, plain, y is not None,
+                    [None if t is None else t.dtype for t in (weight, post, scale_vector)])
+        return (h,) if xn is None else (xn, h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        t, y, w, pw, gate, sv, rstd_x, rstd_y = ctx.saved_tensors
+        scale, eps, plain, has_y, dtypes = ctx.meta
+        dxn, dh = grads if has_y else (None, grads[0])
+        if dxn is None and dh is None:
+            return (None,) * 8
+        need = ctx.needs_input_grad
+        D, dev = t.shape[-1], t.device
+        rows = t.numel() // D
+        dxn = None if dxn is None else dxn.to(t.dtype).contiguous()
+        dh = None if dh is None else dh.to(t.dtype).contiguous()
+        full = has_y and not plain
+        want_x = need[0] or (plain and has_y and need[1])
+        rowwise = lambda on: torch.empty(t.shape, device=dev, dtype=t.dtype) if on else None
+        column = lambda on: torch.zeros(D, device=dev, dtype=torch.float32) if on and not rows \
+            else (torch.empty(D, device=dev, dtype=torch.float32) if on else None)
+        dx = rowwise(want_x)
+        dy = rowwise(full and need[1])
+        dgate = rowwise(gate is not None and need[4])
+        dw = column(need[2])
+        dpost = column(pw is not None and need[3])
+        dscale = column(sv is not None and need[5])
+        if rows:
+            args, _keep = _args(t, y if full else None, gate, w, pw, sv, scale, eps)
+            nbytes = _lib.lib().cyfa_residual_norm_bwd_work_bytes(rows, D)
+            work = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+            P = _lib.ptr
+            with on_device(t):
+                _lib.call("cyfa_residual_norm_bwd", ctypes.byref(args), rstd_x.data_ptr(),
+                          P(rstd_y), P(dxn), P(dh), P(dx), P(dy), P(dgate), P(dw), P(dpost),
+                          P(dscale), work.data_ptr(), ctypes.c_size_t(nbytes), _lib.stream())
+        if plain and has_y and need[1]:
+            dy = dx
+        dw, dpost, dscale = (g if g is None else g.to(d)
+                             for g, d in zip((dw, dpost, dscale), dtypes))
+        return dx if need[0] else None, dy, dw, dpost, dgate, dscale, None, None
+
+
+def residual_norm(x, y, weight, post_weight=None, gate=None, scale=None, eps=1e-6):
+    """Adds a block's branch to the residual stream and normalises the sum:
+
+        z  = y, or RMSNorm(y) * post_weight
+        x' = x + scale * sigmoid(gate) * z
+        h  = RMSNorm(x') * weight
+
+    and returns ``(x', h)``: the new stream and the next branch's input.  ``x``,
+    ``y`` and ``gate`` share one shape [..., D] (D <= 8192) and dtype (bf16 or fp32);
+    ``weight``, ``post_weight`` [D]; ``scale`` a number, a [D] tensor, or None for 1.
+    ``y = None`` is the norm alone (``x'`` is then ``x`` itself).  fp32 arithmetic; x' is rounded to its
+    dtype before it is normalised, as the decoder block keeps it.  Gradients flow
+    to every tensor; those of the [D] parameters are summed over the rows in fp32
+    in a fixed order.  ``gate`` and ``y`` do not broadcast: expand them first
+    (the copy and the gradient's sum are then autograd's).
+    """
+    scale_vector = scale if isinstance(scale, torch.Tensor) else None
+    dtype_code("x", x)
+    if x.dim() < 1 or not 0 < x.shape[-1] <= MAX_WIDTH:
+        raise ValueError(f"x must be [..., D] with 0 < D <= {MAX_WIDTH}, got {tuple(x.shape)}")
+    if y is None and (post_weight is not None or gate is not None or scale is not None):
+        raise ValueError("post_weight, gate and scale act on y, which is None")
+    for name, t in (("y", y), ("gate", gate)):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError(f"{name} must be {x.dtype} of shape {tuple(x.shape)}, got {t.dtype} "
+                             f"of {tuple(t.shape)}")
+    for name, t in (("weight", weight), ("post_weight", post_weight), ("scale", scale_vector)):
+        if t is not None and (t.dim() != 1 or t.shape[0] != x.shape[-1]):
+            raise ValueError(f"{name} must have shape [{x.shape[-1]}], got {tuple(t.shape)}")
+        if t is not None and not t.is_floating_point():
+            raise TypeError(f"{name} must be a floating-point tensor, got {t.dtype}")
+    if x.numel() // x.shape[-1] >= 1 << 31:
+        raise ValueError("at most 2^31 - 1 rows per call")
+    number = 1.0 if scale is None or scale_vector is not None else float(scale)
+    if not (math.isfinite(number) and math.isfinite(eps) and eps >= 0):
+        raise ValueError(f"scale and eps must be finite and eps >= 0, got {scale}, {eps}")
+    same_device(x=x, y=y, weight=weight, post_weight=post_weight, gate=gate, scale=scale_vector)
+    tensors = (x, y, weight, post_weight, gate, scale_vector)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        out = ResidualNormFunction.apply(*tensors, number, float(eps))
+        return (x, out[0]) if y is None else out
+    xn, h, _, _ = _forward(x.detach(), None if y is None else y.detach(), f32(weight),
+                           f32(post_weight), None if gate is None else gate.detach(),
+                           f32(scale_vector), number, float(eps))
+    return x if xn is None else xn, h

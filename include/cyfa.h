@@ -40,7 +40,8 @@ int cyfa_version(void);
 const char* cyfa_strerror(int status);
 
 /* Reads (and, if reset != 0, clears) the device error word of the current
- * device: 0 = no device-side failure; 1 = a bounded wait timed out.
+ * device: 0 = no device-side failure; 1 = a bounded wait timed out; 3 = a token
+ * outside the vocabulary (token_logprobs, embed).
  * Synchronises the device. */
 int cyfa_device_error(int reset);
 
@@ -421,6 +422,102 @@ int cyfa_decode_conv(const void* x, long long x_stride, void* cache_q, void* cac
  * (gate columns first, then up columns), out [rows, mid] bf16; mid % 8 == 0.
  * Replaces: GatedMLP.execute (models/cyfa/modeling_cyfa.py:22-27). */
 int cyfa_swiglu(const void* gu, void* out, int rows, int mid, void* stream);
+
+/* ---------------------------------------------------------------- token log probabilities
+ * log p of one given token per row of logits, the entropy of the row's softmax
+ * and its `top` most likely tokens (0 <= top <= 32, top <= V), ordered by
+ * (logit, then lowest index); dtype of the logits 0 = f32, 1 = bf16, sums in f32.
+ * Replaces: the loss of the causal LM (models/cyfa/modeling_cyfa.py:102-116,
+ * cross entropy over fp32 logits); entropy and alternatives have no counterpart.
+ * Row r of the logits starts at (r / inner) * stride_outer + (r % inner) *
+ * stride_inner elements (0 <= r < rows) and is V contiguous elements; no row
+ * alignment is needed.  tokens [rows] i64: a row whose token is ignore_index has
+ * logp 0 and no gradient from it; any other token outside [0, V) gives NaN, no
+ * gradient and device error 3.  Masked logits (-inf) have probability 0; a row with
+ * no finite logit has logp -inf, entropy 0 and zero gradient.
+ * stats [rows, 2] f32 (row maximum, log of the sum) is kept for the backward;
+ * top_logp / top_tokens [rows, top] may be NULL when top is 0. */
+int cyfa_token_logprobs_fwd(const void* logits, int dtype, long long rows, long long inner,
+                            long long stride_outer, long long stride_inner, int V,
+                            const long long* tokens, long long ignore_index, int top, float* logp,
+                            float* entropy, float* stats, float* top_logp, long long* top_tokens,
+                            void* stream);
+
+/* dlogits [rows, V] (contiguous, the logits' dtype) from the gradients of logp
+ * and entropy ([rows] f32, either may be NULL). */
+int cyfa_token_logprobs_bwd(const void* logits, int dtype, long long rows, long long inner,
+                            long long stride_outer, long long stride_inner, int V,
+                            const long long* tokens, long long ignore_index, const float* stats,
+                            const float* entropy, const float* dlogp, const float* dentropy,
+                            void* dlogits, void* stream);
+
+/* ---------------------------------------------------------------- embedding
+ * out[n] = scale * weight[tokens[n]] (weight [V, D], out [N, D], dtype 0 = f32,
+ * 1 = bf16; tokens i64).  A token outside [0, V) gives a zero row and device
+ * error 3.  Replaces: the embedding of models/cyfa/modeling_cyfa.py:58-69. */
+int cyfa_embed_fwd(const long long* tokens, const void* weight, int dtype, void* out, long long N,
+                   long long V, int D, float scale, void* stream);
+
+/* The whole table's gradient dweight [V, D] (weight's dtype, every row written):
+ * row v is scale times the sum, in f32 and in ascending n, of dout[n] over the
+ * tokens equal to v; the rows of tokens that do not occur and of padding_idx (-1:
+ * none) are zero.  The tokens are sorted first, so the result does not depend on
+ * the order in which CTAs run.  N < 2^31, V < 2^31.  work: 256-byte aligned. */
+size_t cyfa_embed_bwd_work_bytes(long long N, int D);
+int cyfa_embed_bwd(const long long* tokens, const void* dout, int dtype, void* dweight, long long N,
+                   long long V, int D, float scale, long long padding_idx, void* work,
+                   size_t work_bytes, void* stream);
+
+/* ---------------------------------------------------------------- residual norm
+ * A block's residual add with its norms, gate and scale, with gradients:
+ *   z = y or RMSNorm(y) * post_weight;  xn = x + scale * sigmoid(gate) * z;
+ *   h = RMSNorm(xn) * weight
+ * (xn rounded to the tensors' dtype before the norm, as the decoder block keeps
+ * it: models/cyfa/modeling_cyfa.py:52-55,64-69).  x, y, gate [rows, D] of one dtype
+ * (0 = f32, 1 = bf16), row strides in elements; D <= 8192.  Absent (NULL): y (h is
+ * the norm of x, xn is not written), gate, post_weight, scale_vector (then the
+ * number `scale` applies). */
+typedef struct {
+  long long rows;
+  int D, dtype;
+  const void* x;
+  const void* y;
+  const void* gate;
+  long long x_stride, y_stride, gate_stride;
+  const float* weight;       /* [D] */
+  const float* post_weight;  /* [D] or NULL */
+  const float* scale_vector; /* [D] or NULL */
+  float scale;
+  float eps;
+} cyfa_residual_norm_args;
+
+/* xn, h [rows, D] contiguous; rstd_x, rstd_y [rows] f32 kept for the backward
+ * (rstd_y only with post_weight). */
+int cyfa_residual_norm_fwd(const cyfa_residual_norm_args* args, void* xn, void* h, float* rstd_x,
+                           float* rstd_y, void* stream);
+
+/* args->x is the new stream xn here (x itself when y is NULL).  dxn, dh [rows, D]
+ * contiguous, either may be NULL (zero).  Outputs, each may be NULL: dx, dy, dgate
+ * [rows, D] contiguous in the tensors' dtype, dweight, dpost, dscale [D] f32 (sums
+ * over the rows in a fixed order).  work: 16-byte aligned. */
+size_t cyfa_residual_norm_bwd_work_bytes(long long rows, int D);
+int cyfa_residual_norm_bwd(const cyfa_residual_norm_args* args, const float* rstd_x,
+                           const float* rstd_y, const void* dxn, const void* dh, void* dx,
+                           void* dy, void* dgate, float* dweight, float* dpost, float* dscale,
+                           void* work, size_t work_bytes, void* stream);
+
+/* ---------------------------------------------------------------- Newton-Schulz
+ * out [L, m, n] bf16: each matrix of g [L, m, n] (dtype 0 = f32, 1 = bf16)
+ * divided by its Frobenius norm + eps, then `steps` times
+ *   X <- a X + (b A + c A A) X,  A = X X^T   (of the shorter side)
+ * No counterpart in the reference (whose optimizer is AdamW, training/optim.py).
+ * The coefficients have to keep every |entry| of X, A and b A + c A A below 16, as
+ * the usual quintic (3.4445, -4.7750, 2.0315) does.  m, n <= 65536, L <= 65535.
+ * work: 256-byte aligned. */
+size_t cyfa_newton_schulz_work_bytes(int L, int m, int n);
+int cyfa_newton_schulz(const void* g, int dtype, int L, int m, int n, int steps, float a, float b,
+                       float c, float eps, void* out, void* work, size_t work_bytes,
+                       void* stream);
 
 /* ---------------------------------------------------------------- self test
  * C[128,N] = A * B through TMA + tcgen05 (test hook for the UMMA descriptor and
