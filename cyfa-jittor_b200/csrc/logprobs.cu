@@ -29,7 +29,7 @@ struct LogprobParams {
   long long ignore;
   float* logp;              // [rows]
   float* entropy;           // [rows]
-  float2* stats;            // [rows] (m, log s)
+  float2* stats;            // [rows] (m, log s), may be null forward
   float* top_logp;          // [rows, top]
   long long* top_tokens;    // [rows, top]
   int V, top;
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kLpThreads) logprob_fwd_kernel(LogprobParams p
     if (tid == 0) {
       const float h = empty ? 0.f : logs - tot.t / tot.s;
       p.entropy[row] = h < 0.f ? 0.f : h;
-      p.stats[row] = make_float2(tot.m, logs);
+      if (p.stats) p.stats[row] = make_float2(tot.m, logs);
       const long long id = p.tokens[row];
       float lp = 0.f;
       if (id != p.ignore) {
@@ -478,12 +478,12 @@ int cyfa_token_logprobs_fwd(const void* logits, int dtype, long long rows, long 
                             const long long* tokens, long long ignore_index, int top, float* logp,
                             float* entropy, float* stats, float* top_logp, long long* top_tokens,
                             void* stream) {
-  CYFA_REQUIRE(logits && tokens && logp && entropy && stats && (top == 0 || (top_logp && top_tokens)),
+  CYFA_REQUIRE(logits && tokens && logp && entropy && (top == 0 || (top_logp && top_tokens)),
                kNullPointer);
   const int rc = logprob_checks(logits, dtype, rows, inner, stride_outer, stride_inner, V);
   if (rc) return rc;
   CYFA_REQUIRE(top >= 0 && top <= kLpMaxTop && top <= V && rows < (1ll << 27), kBadShape);
-  CYFA_REQUIRE(aligned(tokens, 8) && aligned(stats, 8) && aligned(logp, 4) && aligned(entropy, 4) &&
+  CYFA_REQUIRE(aligned(tokens, 8) && (!stats || aligned(stats, 8)) && aligned(logp, 4) && aligned(entropy, 4) &&
                    (!top || (aligned(top_logp, 4) && aligned(top_tokens, 8))),
                kMisaligned);
   LogprobParams p{};

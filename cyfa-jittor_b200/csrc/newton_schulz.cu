@@ -4,13 +4,20 @@
 //   A = X X^T,   B = b A + c A A,   X <- a X + B X        (each step)
 // which pushes every singular value towards 1.
 //
-// The products run on tcgen05 with fp32 accumulators in TMEM.  Small singular
-// values grow by a = 3.4 a step, and so do rounding errors beside them, so the
-// operands are kept as fp16 pairs hi + lo (22 significant bits) and a product is
-// the three MMAs hi hi + hi lo + lo hi.  X, A and B are stored times 2^12, which
-// keeps the lo parts of small entries above fp16's underflow and leaves room up
-// to |entry| < 16.  A and B are symmetric: only the tiles on and below the
-// diagonal are computed, the others are written as their mirror images.
+// The products run on tcgen05 (CTA pairs) with fp32 accumulators in TMEM.  X, A
+// and B are kept as fp16 pairs hi + lo (22 significant bits), stored times 2^12:
+// that keeps the lo parts of small entries above fp16's underflow and leaves room
+// up to |entry| < 16.  A product is the three MMAs hi hi + hi lo + lo hi where its
+// rounding would show, one MMA hi hi where it does not: a X + B X cancels to a
+// tenth of its terms once the singular values are near 1, so in the last three
+// steps A A and B X take all three; A = X X^T (whose error is not cancelled
+// against anything) and every product of the earlier steps take one.  Simulated
+// in 64 bits on Gaussian, low-rank and graded matrices this is within 1.5e-4 to
+// 6e-4 relative of the exact iteration, a third of the bf16 rounding of the
+// result (1.7e-3); one MMA everywhere is up to 2.8e-3 off, three everywhere 8e-7,
+// at 1.6 times the MMAs.
+// A and B are symmetric: only the tiles on and below the diagonal are computed,
+// the others are written as their mirror images.
 #include <cuda_fp16.h>
 
 #include "cyfa_common.cuh"
@@ -18,8 +25,16 @@
 namespace cyfa {
 
 constexpr float kNsScale = 4096.f;  // 2^12
-constexpr int kNsEpiWarps = 8;
-constexpr int kNsThreads = (kNsEpiWarps + 2) * 32;
+template <int PROD>
+constexpr int ns_epi_warps() {
+  return PROD == 3 ? 8 : 16;
+}
+template <int PROD>
+constexpr int ns_threads() {
+  return (ns_epi_warps<PROD>() + 2) * 32;
+}
+constexpr int kNsFullSteps = 3;  // last steps with three-MMA products
+constexpr int kNsTile = 256;  // rows and columns of a CTA pair's tile
 
 enum NsMode : int {
   kNsGram = 0,    // D = acc
@@ -30,26 +45,28 @@ enum NsMode : int {
 
 struct NsGemmParams {
   int L, M, cols, K;        // D [L, M, cols] = contraction over K
-  int tiles_m, tiles_n;
+  int tiles_m;
+  int nunits, per;          // tiles in all, tiles of one matrix
   float alpha, beta;
-  const __half *ch, *cl;    // C pair, layout of D
-  __half *dh, *dl;          // D pair [L, M, ld]
-  long long ld;             // row stride of C and D (a multiple of 8)
   __nv_bfloat16* out;       // kNsLast
   int tall;                 // out is [L, cols, M]
 };
 
-template <int BN>
+// Per stage and CTA: 128 rows of A and 128 of B, 64 contraction columns each, hi
+// and (with three products) lo.
+constexpr int kNsPart = 128 * 128;
+constexpr int kNsSlot = 32 * 64;  // a finishing warp's block: 32 rows x 32 columns of 16 bits
+template <int PROD>
 constexpr int ns_stage_bytes() {
-  return 2 * 128 * 128 + 2 * BN * 128;  // Ah, Al [128 x 64], Bh, Bl [BN x 64]
+  return (PROD == 3 ? 4 : 2) * kNsPart;
 }
-template <int BN>
+template <int PROD>
 constexpr int ns_stages() {
-  return BN == 256 ? 2 : 3;
+  return PROD == 3 ? 3 : 5;
 }
-template <int BN>
+template <int PROD>
 constexpr int ns_smem() {
-  return ns_stages<BN>() * ns_stage_bytes<BN>() + 1024;
+  return ns_stages<PROD>() * ns_stage_bytes<PROD>() + ns_epi_warps<PROD>() * 2 * kNsSlot + 1024;
 }
 
 // fp16 x fp16 -> fp32
@@ -58,23 +75,20 @@ __host__ __device__ constexpr uint32_t ns_idesc(int M, int N, int b_mn) {
 }
 
 // Unit u -> (matrix, row tile, column tile).  Symmetric products skip the tiles
-// above the diagonal: row tile i has the column tiles j with j BN/128 <= i.
+// above the diagonal: row tile i has the column tiles 0 .. i.
 struct NsTile {
   int l, ti, tj;
 };
-template <int BN, bool SYM>
-__device__ __forceinline__ NsTile ns_tile(const NsGemmParams& p, int u, int per) {
+template <bool SYM>
+__device__ __forceinline__ NsTile ns_tile(const NsGemmParams& p, int u) {
   NsTile t;
-  t.l = u / per;
-  int r = u - t.l * per;
+  t.l = u / p.per;
+  int r = u - t.l * p.per;
   if (SYM) {
-    constexpr int nb = BN / 128;
     t.ti = 0;
-    while (true) {
-      const int w = t.ti / nb + 1;
-      if (r < w) break;
-      r -= w;
+    while (r > t.ti) {
       ++t.ti;
+      r -= t.ti;
     }
     t.tj = r;
   } else {
@@ -84,28 +98,158 @@ __device__ __forceinline__ NsTile ns_tile(const NsGemmParams& p, int u, int per)
   return t;
 }
 
-__device__ __forceinline__ uint32_t pack_half2(__half a, __half b) {
-  return uint32_t(__half_as_ushort(a)) | (uint32_t(__half_as_ushort(b)) << 16);
+// ------------------------------------------------ finishing a tile
+// A finishing warp's blocks of 32 x 32 16-bit entries in shared memory, laid out as
+// the 64-byte TMA swizzle: 4 chunks of 16 bytes a row.  A lane reads and writes its
+// own row; memory is reached by TMA.  (Going to memory from the registers, by rows
+// or through a warp transposition, cost more load/store issue than the tile's
+// MMAs take: 209 us against 140 for B X on 24 matrices of 1024 x 2816.)
+__device__ __forceinline__ uint32_t ns_slot(uint32_t block, int row, int chunk) {
+  return block + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+}
+// v += beta * the block's row `lane`
+__device__ __forceinline__ void ns_add(uint32_t block, float beta, float (&v)[32]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint4 u = ld_shared_v4(ns_slot(block, lane, c));
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 x = __half22float2(h[e]);
+      v[8 * c + 2 * e] = fmaf(beta, x.x, v[8 * c + 2 * e]);
+      v[8 * c + 2 * e + 1] = fmaf(beta, x.y, v[8 * c + 2 * e + 1]);
+    }
+  }
+}
+// row: the lane's 32 entries, two to a word
+__device__ __forceinline__ void ns_put(uint32_t block, const uint32_t (&row)[16]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    st_shared_v4(ns_slot(block, lane, c), row[4 * c], row[4 * c + 1], row[4 * c + 2],
+                 row[4 * c + 3]);
+}
+// The block transposed: 8 x 8 pieces read with their transposition into t, then
+// written back as the pieces of the transposed block.
+__device__ __forceinline__ void ns_read_transposed(uint32_t block, uint32_t (&t)[16]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(t[4 * g]), "=r"(t[4 * g + 1]), "=r"(t[4 * g + 2]), "=r"(t[4 * g + 3])
+                 : "r"(ns_slot(block, lane, g))
+                 : "memory");
+}
+__device__ __forceinline__ void ns_write_transposed(uint32_t block, const uint32_t (&t)[16]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                     ns_slot(block, 8 * g + (lane & 7), lane >> 3)),
+                 "r"(t[4 * g]), "r"(t[4 * g + 1]), "r"(t[4 * g + 2]), "r"(t[4 * g + 3])
+                 : "memory");
+}
+// The block to rows of dst (stride ld), 8 rows x 64 bytes at a time or, for rows at
+// any alignment, one row at a time; rows from `rows` and columns from `cols` on are
+// left out.
+__device__ __forceinline__ void ns_store(uint32_t block, __nv_bfloat16* dst, long long ld, int rows,
+                                         int cols, bool aligned16) {
+  const int lane = threadIdx.x & 31;
+  if (aligned16) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = 8 * k + (lane >> 2), c = lane & 3;
+      const uint4 u = ld_shared_v4(ns_slot(block, r, c));
+      if (r < rows && c * 8 < cols) *reinterpret_cast<uint4*>(dst + r * ld + c * 8) = u;
+    }
+  } else {
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+      uint16_t u;
+      asm volatile("ld.shared.u16 %0, [%1];"
+                   : "=h"(u)
+                   : "r"(ns_slot(block, r, lane >> 3) + (lane & 7) * 2));
+      if (r < rows && lane < cols) dst[r * ld + lane] = __ushort_as_bfloat16(u);
+    }
+  }
+}
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// hi parts of v packed into w, v becomes what they leave
+__device__ __forceinline__ void ns_split_row(float (&v)[32], uint32_t (&w)[16]) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    w[e] = pack_half2(v[2 * e], v[2 * e + 1]);
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+    v[2 * e] -= h.x;
+    v[2 * e + 1] -= h.y;
+  }
 }
 
-// Persistent; warp 8 loads (one lane), warp 9 issues the MMAs (one lane), warps
-// 0-7 finish tiles from the two TMEM accumulators: warp w reads lane quadrant
-// w & 3 (32 rows) and column half w >> 2.
-template <int BN, int MODE>
-__global__ void __launch_bounds__(kNsThreads, 1)
+// ------------------------------------------------ CTA pair (cta_group::2)
+// Tile load into this CTA's shared memory, completion signalled on the barrier
+// at the cluster address `bar` (the leader's).
+__device__ __forceinline__ void pair_load_3d(void* dst, const void* tmap, uint32_t bar, int x, int y,
+                                             int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(tmap), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void pair_umma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                          uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+// Arrives on the barrier at this address in both CTAs when the MMAs issued so far
+// are done.
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%0], %1;" ::"r"(smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+__device__ __forceinline__ void cluster_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// TMA addresses of the finishing warps: C and D as pairs of 32 x 32 blocks.
+struct NsEpiMaps {
+  CUtensorMap ch, cl, dh, dl;
+};
+
+// Persistent CTA pairs; a pair's tile is 256 x 256, CTA r of it holds rows 128 r ..
+// of the result (in its TMEM) and of A, and columns 128 r .. of B.  One warp
+// loads (one lane), one of the leader's issues the MMAs of both CTAs (one lane), the
+// EPI others finish the tile from one of the two TMEM accumulators while the next
+// tile is computed into the other: warp w reads lane quadrant w & 3 (32 rows) and
+// the columns (1024 / EPI) (w >> 2) .., 32 at a time.  PROD: MMAs per product (3: hi and lo parts).
+template <int PROD, int MODE>
+__global__ void __launch_bounds__(ns_threads<PROD>(), 1)
     ns_gemm_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_constant__ CUtensorMap map_al,
                    const __grid_constant__ CUtensorMap map_bh, const __grid_constant__ CUtensorMap map_bl,
-                   NsGemmParams p, int nunits, int per) {
+                   const __grid_constant__ NsEpiMaps em, NsGemmParams p) {
   constexpr bool SYM = MODE == kNsGram || MODE == kNsPoly;
-  constexpr int kStage = ns_stage_bytes<BN>(), kStages = ns_stages<BN>();
+  constexpr int kStage = ns_stage_bytes<PROD>(), kStages = ns_stages<PROD>();
+  constexpr int kEpi = ns_epi_warps<PROD>();
+  constexpr int kB = kStage / 2;  // B parts follow the A parts
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   __shared__ __align__(8) uint64_t full[kStages], empty[kStages], t_full[2], t_empty[2];
+  __shared__ __align__(8) uint64_t c_full[kEpi];
   __shared__ uint32_t tmem_base;
   __shared__ int s_abort;
   volatile int* abort_flag = &s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = int(cluster_rank()), pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 1);
@@ -113,33 +257,36 @@ __global__ void __launch_bounds__(kNsThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&t_full[i], 1);
-      mbar_init(&t_empty[i], kNsEpiWarps);
+      mbar_init(&t_empty[i], 2 * kEpi);
     }
+    for (int i = 0; i < kEpi; ++i) mbar_init(&c_full[i], 1);
     s_abort = 0;
     mbar_fence_init();
     prefetch_tmap(&map_ah);
-    prefetch_tmap(&map_al);
     prefetch_tmap(&map_bh);
-    prefetch_tmap(&map_bl);
   }
   if (warp == 0) {
-    tmem_alloc(&tmem_base, 2 * BN);
-    tmem_relinquish();
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&tmem_base)),
+                 "r"(2 * kNsTile));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync_all();  // the peer's barriers are ready
   tc_fence_after();
   pdl_wait();
   pdl_trigger();
   const uint32_t tmem = tmem_base;
   const int nk = (p.K + 63) / 64;
 
-  if (warp == kNsEpiWarps) {
+  if (warp == kEpi) {
     if (lane == 0) {
       int q = 0;
       bool ok = true;
-      for (int u = blockIdx.x; ok && u < nunits && !*abort_flag; u += gridDim.x) {
-        const NsTile t = ns_tile<BN, SYM>(p, u, per);
+      for (int u = pair; ok && u < p.nunits && !*abort_flag; u += npairs) {
+        const NsTile t = ns_tile<SYM>(p, u);
+        const int ra = t.ti * kNsTile + rank * 128, cb = t.tj * kNsTile + rank * 128;
         for (int k = 0; k < nk; ++k, ++q) {
           const int s = q % kStages;
           if (q >= kStages && !mbar_wait(&empty[s], ((q / kStages) - 1) & 1)) {
@@ -147,43 +294,45 @@ __global__ void __launch_bounds__(kNsThreads, 1)
             break;
           }
           uint8_t* st = smem + s * kStage;
-          mbar_expect_tx(&full[s], kStage);
-          tma_load_3d(st, &map_ah, &full[s], 64 * k, t.ti * 128, t.l);
-          tma_load_3d(st + 16384, &map_al, &full[s], 64 * k, t.ti * 128, t.l);
-          uint8_t* sb = st + 32768;
+          const uint32_t bar = cluster_map(smem_u32(&full[s]), 0);
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * kStage);  // both CTAs' bytes
+          pair_load_3d(st, &map_ah, bar, 64 * k, ra, t.l);
+          if (PROD == 3) pair_load_3d(st + kNsPart, &map_al, bar, 64 * k, ra, t.l);
           if (SYM) {
-            tma_load_3d(sb, &map_bh, &full[s], 64 * k, t.tj * BN, t.l);
-            tma_load_3d(sb + BN * 128, &map_bl, &full[s], 64 * k, t.tj * BN, t.l);
+            pair_load_3d(st + kB, &map_bh, bar, 64 * k, cb, t.l);
+            if (PROD == 3) pair_load_3d(st + kB + kNsPart, &map_bl, bar, 64 * k, cb, t.l);
           } else {
 #pragma unroll
-            for (int c = 0; c < BN / 64; ++c) {
-              tma_load_3d(sb + c * 8192, &map_bh, &full[s], t.tj * BN + 64 * c, 64 * k, t.l);
-              tma_load_3d(sb + BN * 128 + c * 8192, &map_bl, &full[s], t.tj * BN + 64 * c, 64 * k,
-                          t.l);
+            for (int c = 0; c < 2; ++c) {
+              pair_load_3d(st + kB + c * 8192, &map_bh, bar, cb + 64 * c, 64 * k, t.l);
+              if (PROD == 3)
+                pair_load_3d(st + kB + kNsPart + c * 8192, &map_bl, bar, cb + 64 * c, 64 * k, t.l);
             }
           }
         }
       }
       if (!ok) *abort_flag = 1;
-      // every issued copy lands before shared memory goes away
-      for (int j = q > kStages ? q - kStages : 0; j < q; ++j)
-        mbar_wait(&full[j % kStages], (j / kStages) & 1);
+      // every copy lands before shared memory goes away: the leader sees both
+      // CTAs' copies, the peer stays until the cluster barrier below
+      if (rank == 0)
+        for (int j = q > kStages ? q - kStages : 0; j < q; ++j)
+          mbar_wait(&full[j % kStages], (j / kStages) & 1);
     }
-  } else if (warp == kNsEpiWarps + 1) {
-    if (lane == 0) {
-      const uint32_t idesc = ns_idesc(128, BN, SYM ? 0 : 1);
+  } else if (warp == kEpi + 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = ns_idesc(kNsTile, kNsTile, SYM ? 0 : 1);
       int q = 0, i = 0;
       uint64_t* last_bar = nullptr;
       uint32_t last_par = 0;
       bool ok = true;
-      for (int u = blockIdx.x; ok && u < nunits && !*abort_flag; u += gridDim.x, ++i) {
+      for (int u = pair; ok && u < p.nunits && !*abort_flag; u += npairs, ++i) {
         const int b = i & 1;
         if (i >= 2 && !mbar_wait(&t_empty[b], ((i >> 1) - 1) & 1)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t acc = tmem + b * BN;
+        const uint32_t acc = tmem + b * kNsTile;
         for (int k = 0; k < nk; ++k, ++q) {
           const int s = q % kStages;
           if (!mbar_wait(&full[s], (q / kStages) & 1)) {
@@ -191,23 +340,28 @@ __global__ void __launch_bounds__(kNsThreads, 1)
             break;
           }
           tc_fence_after();
-          const uint32_t ah = smem_u32(smem + s * kStage), al = ah + 16384, bh = ah + 32768,
-                         bl = bh + BN * 128;
+          const uint32_t ah = smem_u32(smem + s * kStage), bh = ah + kB;
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
-            const uint64_t dah = kmaj_desc(ah, 128, ks), dal = kmaj_desc(al, 128, ks);
-            const uint64_t dbh = SYM ? kmaj_desc(bh, BN, ks) : mnmaj_desc(bh, 64, ks);
-            const uint64_t dbl = SYM ? kmaj_desc(bl, BN, ks) : mnmaj_desc(bl, 64, ks);
-            umma_bf16(acc, dal, dbh, idesc, k > 0 || ks > 0);
-            umma_bf16(acc, dah, dbl, idesc, 1);
-            umma_bf16(acc, dah, dbh, idesc, 1);
+            const uint64_t dah = kmaj_desc(ah, 128, ks);
+            const uint64_t dbh = SYM ? kmaj_desc(bh, 128, ks) : mnmaj_desc(bh, 64, ks);
+            if (PROD == 3) {
+              const uint64_t dal = kmaj_desc(ah + kNsPart, 128, ks);
+              const uint64_t dbl = SYM ? kmaj_desc(bh + kNsPart, 128, ks)
+                                       : mnmaj_desc(bh + kNsPart, 64, ks);
+              pair_umma(acc, dal, dbh, idesc, k > 0 || ks > 0);
+              pair_umma(acc, dah, dbl, idesc, 1);
+              pair_umma(acc, dah, dbh, idesc, 1);
+            } else {
+              pair_umma(acc, dah, dbh, idesc, k > 0 || ks > 0);
+            }
           }
-          umma_commit(&empty[s]);
+          pair_commit(&empty[s]);
           last_bar = &empty[s];
           last_par = (q / kStages) & 1;
         }
         if (!ok) break;
-        umma_commit(&t_full[b]);
+        pair_commit(&t_full[b]);
         last_bar = &t_full[b];
         last_par = (i >> 1) & 1;
       }
@@ -215,135 +369,181 @@ __global__ void __launch_bounds__(kNsThreads, 1)
       if (last_bar) mbar_wait(last_bar, last_par);  // all issued MMAs are done
     }
   } else {
-    const int quad = warp & 3, half = warp >> 2;
+    constexpr int kCols = 1024 / kEpi;  // of this warp
+    const int quad = warp & 3, group = warp >> 2;
+    uint8_t* slot = smem + kStages * kStage + warp * 2 * kNsSlot;
+    const uint32_t bh = smem_u32(slot), bl = bh + kNsSlot;  // hi and lo block
+    constexpr bool HAS_C = MODE != kNsGram;
+    constexpr float kDown = 1.f / kNsScale;
+    const float al = (MODE == kNsPoly ? p.alpha : 1.f) * kDown;
+    bool stores = false;  // bulk stores issued (lane 0)
+    int cq = 0;           // C blocks so far
+    auto fetch_c = [&](int c, int r, int l) {
+      if (lane == 0) {
+        if (stores) bulk_wait_read_all();  // the blocks' last contents have left
+        mbar_expect_tx(&c_full[warp], 2 * kNsSlot);
+        tma_load_3d(slot, &em.ch, &c_full[warp], c, r, l);
+        tma_load_3d(slot + kNsSlot, &em.cl, &c_full[warp], c, r, l);
+      }
+    };
     int i = 0;
-    for (int u = blockIdx.x; u < nunits; u += gridDim.x, ++i) {
+    for (int u = pair; u < p.nunits; u += npairs, ++i) {
       const int b = i & 1;
+      const NsTile t = ns_tile<SYM>(p, u);
+      const int r0 = t.ti * kNsTile + rank * 128 + quad * 32;
+      const int col0 = t.tj * kNsTile + group * kCols;
+      const int rows = min(32, p.M - r0);  // of this warp
+      const bool work = rows > 0 && col0 < p.cols;
+      // C does not depend on the products: its first block is on the way while
+      // they finish
+      if (HAS_C && work) fetch_c(col0, r0, t.l);
       const bool got =
           __all_sync(0xffffffffu, *abort_flag == 0 && mbar_wait(&t_full[b], (i >> 1) & 1));
       if (!got) {
         *abort_flag = 1;
+        if (HAS_C && work) mbar_wait(&c_full[warp], cq & 1);  // the copies land first
         break;
       }
       tc_fence_after();
-      const NsTile t = ns_tile<BN, SYM>(p, u, per);
-      const int r = t.ti * 128 + quad * 32 + lane;
-      const bool row_in = r < p.M;
-      const size_t mat = size_t(t.l) * p.M * p.ld;
-      constexpr int nb = BN / 128;
 #pragma unroll 1
-      for (int cc = 0; cc < BN / 64; ++cc) {
-        const int cl0 = half * (BN / 2) + 32 * cc;  // column in the tile
-        const int c0 = t.tj * BN + cl0;
+      for (int cc = 0; cc < kCols / 32; ++cc) {
+        const int c0 = col0 + 32 * cc;
+        if (!work || c0 >= p.cols) break;  // the same for the whole warp
         float v[32];
-        tmem_ld32(tmem + ((quad * 32) << 16) + b * BN + cl0, v);
-        if (c0 >= p.cols) continue;  // the same for the whole warp
-        const size_t row_at = mat + size_t(row_in ? r : 0) * p.ld + c0;
-        if (MODE == kNsGram) {
+        tmem_ld32(tmem + ((quad * 32) << 16) + b * kNsTile + group * kCols + 32 * cc, v);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] *= 1.f / kNsScale;
-        } else {
-          const float al = MODE == kNsPoly ? p.alpha / kNsScale : 1.f / kNsScale;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            if (row_in && c0 + 8 * g < p.ld) {
-              const uint4 uh = *reinterpret_cast<const uint4*>(p.ch + row_at + 8 * g);
-              const uint4 ul = *reinterpret_cast<const uint4*>(p.cl + row_at + 8 * g);
-              const __half2* hh = reinterpret_cast<const __half2*>(&uh);
-              const __half2* hl = reinterpret_cast<const __half2*>(&ul);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 x = __half22float2(hh[e]), y = __half22float2(hl[e]);
-                v[8 * g + 2 * e] = fmaf(p.beta, x.x + y.x, v[8 * g + 2 * e] * al);
-                v[8 * g + 2 * e + 1] = fmaf(p.beta, x.y + y.y, v[8 * g + 2 * e + 1] * al);
-              }
-            }
+        for (int e = 0; e < 32; ++e) v[e] *= al;
+        if (HAS_C) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&c_full[warp], cq & 1))) {
+            *abort_flag = 1;
+            break;
           }
+          ++cq;
+          ns_add(bh, p.beta, v);
+          ns_add(bl, p.beta, v);
+        } else {
+          if (lane == 0 && stores) bulk_wait_read_all();
+          __syncwarp();
         }
+        uint32_t w[16];
         if (MODE == kNsLast) {
           if (p.tall) {
-            __nv_bfloat16* o = p.out + size_t(t.l) * p.cols * p.M + size_t(c0) * p.M + r;
+            __nv_bfloat16* o = p.out + (size_t(t.l) * p.cols + c0) * p.M + r0 + lane;
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (row_in && c0 + e < p.cols)
-                o[size_t(e) * p.M] = __float2bfloat16_rn(v[e] * (1.f / kNsScale));
-          } else if (row_in) {
-            __nv_bfloat16* o = p.out + (size_t(t.l) * p.M + r) * p.cols + c0;
-            if (p.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0) {
+              if (lane < rows && c0 + e < p.cols)
+                o[size_t(e) * p.M] = __float2bfloat16_rn(v[e] * kDown);
+          } else {
 #pragma unroll
-              for (int g = 0; g < 4; ++g)
-                if (c0 + 8 * g < p.cols) {
-                  uint32_t w[4];
-#pragma unroll
-                  for (int e = 0; e < 4; ++e)
-                    w[e] = pack_bf16(v[8 * g + 2 * e] * (1.f / kNsScale),
-                                     v[8 * g + 2 * e + 1] * (1.f / kNsScale));
-                  *reinterpret_cast<uint4*>(o + 8 * g) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (c0 + e < p.cols) o[e] = __float2bfloat16_rn(v[e] * (1.f / kNsScale));
-            }
+            for (int e = 0; e < 16; ++e) w[e] = pack_bf16(v[2 * e] * kDown, v[2 * e + 1] * kDown);
+            ns_put(bh, w);
+            __syncwarp();
+            ns_store(bh, p.out + (size_t(t.l) * p.M + r0) * p.cols + c0, p.cols, rows, p.cols - c0,
+                     p.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0);
           }
+          fence_async_smem();  // the next C block overwrites what was read here
+          __syncwarp();
         } else {
-          __half hi[32], lo[32];
+          // hi parts, then what they leave as lo parts
+          ns_split_row(v, w);
+          ns_put(bh, w);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            hi[e] = __float2half_rn(v[e]);
-            lo[e] = __float2half_rn(v[e] - __half2float(hi[e]));
+          for (int e = 0; e < 16; ++e) w[e] = pack_half2(v[2 * e], v[2 * e + 1]);
+          ns_put(bl, w);
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d(&em.dh, slot, c0, r0, t.l);
+            tma_store_3d(&em.dl, slot + kNsSlot, c0, r0, t.l);
+            bulk_commit();
+            stores = true;
           }
-          if (row_in) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-              if (c0 + 8 * g < p.ld) {
-                uint32_t wh[4], wl[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  wh[e] = pack_half2(hi[8 * g + 2 * e], hi[8 * g + 2 * e + 1]);
-                  wl[e] = pack_half2(lo[8 * g + 2 * e], lo[8 * g + 2 * e + 1]);
-                }
-                *reinterpret_cast<uint4*>(p.dh + row_at + 8 * g) = make_uint4(wh[0], wh[1], wh[2], wh[3]);
-                *reinterpret_cast<uint4*>(p.dl + row_at + 8 * g) = make_uint4(wl[0], wl[1], wl[2], wl[3]);
-              }
-          }
-          // the mirror image, where no tile of its own computes it
-          if (SYM && c0 / 128 < t.ti / nb * nb && row_in) {
-            const size_t at = mat + size_t(c0) * p.ld + r;
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              p.dh[at + size_t(e) * p.ld] = hi[e];
-              p.dl[at + size_t(e) * p.ld] = lo[e];
+          if (SYM && t.tj < t.ti) {
+            // the mirror image of a tile below the diagonal
+            uint32_t m[16];
+            ns_read_transposed(bh, w);
+            ns_read_transposed(bl, m);
+            if (lane == 0) bulk_wait_read_all();
+            __syncwarp();
+            ns_write_transposed(bh, w);
+            ns_write_transposed(bl, m);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(&em.dh, slot, r0, c0, t.l);
+              tma_store_3d(&em.dl, slot + kNsSlot, r0, c0, t.l);
+              bulk_commit();
             }
           }
         }
+        if (HAS_C && cc + 1 < kCols / 32 && c0 + 32 < p.cols) fetch_c(c0 + 32, r0, t.l);
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&t_empty[b]);
+      if (lane == 0) cluster_arrive(cluster_map(smem_u32(&t_empty[b]), 0));
     }
+    if (lane == 0 && stores) bulk_wait_all();
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync_all();  // neither CTA leaves while the other may signal or read it
   if (warp == 0) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * BN);
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(2 * kNsTile));
   }
 }
 
-// Partial sums of squares, in 64 bits: fp32 gradients may be as large as 1e38.
+// Partial sums of squares: 8 entries at a time in fp32, the sums of those in 64
+// bits.  Eight whose fp32 sum overflowed or may have lost squares below the
+// normal range are redone in 64 bits (fp32 gradients reach 1e38).
 constexpr int kNsNormParts = 64;
+constexpr int kNsNormThreads = 512;
 template <typename T>
-__global__ void __launch_bounds__(256) ns_norm_kernel(const T* g, long long per, double* part) {
+__global__ void __launch_bounds__(kNsNormThreads) ns_norm_kernel(const T* g, long long per, double* part) {
+  constexpr int N = 16 / sizeof(T);
   pdl_wait();
   pdl_trigger();
-  __shared__ double red[8];
+  __shared__ double red[kNsNormThreads / 32];
   const T* x = g + (long long)blockIdx.y * per;
   double s = 0.0;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < per;
-       i += (long long)gridDim.x * 256) {
-    const double v = double(float(x[i]));
-    s += v * v;
+  const long long step = (long long)gridDim.x * kNsNormThreads;
+  const long long i0 = (long long)blockIdx.x * kNsNormThreads + threadIdx.x;
+  auto add = [&](const float* f, int n) {
+    float q = 0.f;
+    for (int i = 0; i < n; ++i) q = fmaf(f[i], f[i], q);
+    if (q > 1e-30f && q < 1e30f) {
+      s += double(q);
+    } else {
+      for (int i = 0; i < n; ++i) s += double(f[i]) * double(f[i]);
+    }
+  };
+  const bool vector = per % N == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
+  if (vector) {
+    const uint4* v = reinterpret_cast<const uint4*>(x);
+    const long long n = per / N;
+    long long i = i0;
+    for (; i + 3 * step < n; i += 4 * step) {
+      uint4 u[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) u[k] = v[i + k * step];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float f[N];
+        LpVec<T>::unpack(u[k], f);
+        add(f, N);
+      }
+    }
+    for (; i < n; i += step) {
+      float f[N];
+      LpVec<T>::unpack(v[i], f);
+      add(f, N);
+    }
+  } else {
+    for (long long i = i0; i < per; i += step) {
+      const float f = float(x[i]);
+      add(&f, 1);
+    }
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -351,54 +551,88 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(const T* g, long long per,
   __syncthreads();
   if (threadIdx.x == 0) {
     s = 0.0;
-    for (int w = 0; w < 8; ++w) s += red[w];
+    for (int w = 0; w < kNsNormThreads / 32; ++w) s += red[w];
     part[blockIdx.y * kNsNormParts + blockIdx.x] = s;
   }
 }
 
-// X0 times 2^12 as an fp16 pair, transposed when G is tall: 32 x 32 tiles of G.
+// X0 times 2^12 as an fp16 pair, transposed when G is tall: 64 x 64 tiles of G.
 template <typename T>
 __global__ void __launch_bounds__(256)
     ns_split_kernel(const T* g, int m, int n, const double* part, int parts, float eps, __half* xh,
                     __half* xl, long long ld, int tall) {
   pdl_wait();
   pdl_trigger();
-  __shared__ float tile[32][33];
-  __shared__ double s_inv;
-  if (threadIdx.x == 0) {
+  __shared__ float tile[64][65];
+  __shared__ float s_scale[2];
+  const int tid = threadIdx.x;
+  if (tid < 32) {
     double s = 0.0;
-    for (int i = 0; i < parts; ++i) s += part[blockIdx.z * kNsNormParts + i];
-    s_inv = double(kNsScale) / (sqrt(s) + double(eps));
+    for (int i = tid; i < parts; i += 32) s += part[blockIdx.z * kNsNormParts + i];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (tid == 0) {
+      // the factor as two of fp32's range: its own may be below it
+      const double inv = double(kNsScale) / (sqrt(s) + double(eps));
+      int e;
+      const double f = frexp(inv, &e);
+      s_scale[0] = float(ldexp(1.0, e / 2));
+      s_scale[1] = float(ldexp(f, e - e / 2));
+    }
   }
-  __syncthreads();
-  const double inv = s_inv;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32;
+  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
   const T* src = g + (long long)blockIdx.z * m * n;
-  const int M = tall ? n : m, N = tall ? m : n;
-  __half* oh = xh + (long long)blockIdx.z * M * ld;
-  __half* ol = xl + (long long)blockIdx.z * M * ld;
-  for (int k = 0; k < 4; ++k) {
-    const int r = r0 + ty + 8 * k, c = c0 + tx;
-    const float v = r < m && c < n ? float(double(float(src[(long long)r * n + c])) * inv) : 0.f;
-    if (tall) {
-      tile[ty + 8 * k][tx] = v;
-    } else if (r < M && c < N) {
-      const __half hi = __float2half_rn(v);
-      oh[(long long)r * ld + c] = hi;
-      ol[(long long)r * ld + c] = __float2half_rn(v - __half2float(hi));
+  const bool vector = n % 8 == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
+  // 8 columns x 2 rows of the tile per thread
+  const int tr = tid >> 3, tc = (tid & 7) * 8;
+  float f[2][8];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int r = r0 + tr + 32 * k, c = c0 + tc;
+    const T* q = src + (long long)r * n + c;
+    if (vector && r < m && c < n) {
+      constexpr int N = 16 / sizeof(T);
+#pragma unroll
+      for (int j = 0; j < 8 / N; ++j)
+        LpVec<T>::unpack(*reinterpret_cast<const uint4*>(q + j * N), f[k] + j * N);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[k][i] = r < m && c + i < n ? float(q[i]) : 0.f;
     }
   }
-  if (!tall) return;
   __syncthreads();
-  for (int k = 0; k < 4; ++k) {
-    const int r = c0 + ty + 8 * k, c = r0 + tx;  // of X
-    if (r < M && c < N) {
-      const float v = tile[tx][ty + 8 * k];
-      const __half hi = __float2half_rn(v);
-      oh[(long long)r * ld + c] = hi;
-      ol[(long long)r * ld + c] = __float2half_rn(v - __half2float(hi));
+  const float a = s_scale[0], b = s_scale[1];
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[k][i] = f[k][i] * a * b;
+  if (tall) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) tile[tr + 32 * k][tc + i] = f[k][i];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[k][i] = tile[tc + i][tr + 32 * k];
+  }
+  const int M = tall ? n : m;
+  const int xr = tall ? c0 : r0, xc = tall ? r0 : c0;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int r = xr + tr + 32 * k, c = xc + tc;
+    if (r >= M || c >= ld) continue;
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      h[e] = pack_half2(f[k][2 * e], f[k][2 * e + 1]);
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
+      l[e] = pack_half2(f[k][2 * e] - x.x, f[k][2 * e + 1] - x.y);
     }
+    const long long o = ((long long)blockIdx.z * M + r) * ld + c;
+    *reinterpret_cast<uint4*>(xh + o) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(xl + o) = make_uint4(l[0], l[1], l[2], l[3]);
   }
 }
 
@@ -449,32 +683,31 @@ struct NsWork {
   }
 };
 
-// [L, rows, cols] with row stride ld; box {64, box_rows, 1}
+// [L, rows, cols] with row stride ld; box {box_cols, box_rows, 1} of 64 columns (128-byte
+// swizzle) or 32 (64-byte swizzle)
 static int ns_tmap(CUtensorMap* m, const __half* base, long long L, int rows, int cols, long long ld,
-                   int box_rows) {
+                   int box_cols, int box_rows) {
   const uint64_t dims[3] = {uint64_t(cols), uint64_t(rows), uint64_t(L)};
   const uint64_t strides[2] = {uint64_t(ld) * 2, uint64_t(ld) * rows * 2};
-  const uint32_t box[3] = {64, uint32_t(box_rows), 1};
-  return make_tmap_bf16(m, base, 3, dims, strides, box);  // 16-bit elements; the type only names the fill
+  const uint32_t box[3] = {uint32_t(box_cols), uint32_t(box_rows), 1};
+  // 16-bit elements; the type only names the fill
+  return make_tmap_bf16(m, base, 3, dims, strides, box,
+                        box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-template <int BN, int MODE>
-static void ns_launch(const CUtensorMap& ah, const CUtensorMap& al, const CUtensorMap& bh,
-                      const CUtensorMap& bl, NsGemmParams p, cudaStream_t s) {
+template <int PROD, int MODE>
+static void ns_launch(const CUtensorMap (&a)[2], const CUtensorMap (&b)[2], const CUtensorMap (&c)[2],
+                      const CUtensorMap (&d)[2], NsGemmParams p, cudaStream_t s) {
   constexpr bool SYM = MODE == kNsGram || MODE == kNsPoly;
-  constexpr int nb = BN / 128;
-  p.tiles_m = (p.M + 127) / 128;
-  p.tiles_n = (p.cols + BN - 1) / BN;
-  int per = p.tiles_m * p.tiles_n;
-  if (SYM) {
-    per = 0;
-    for (int i = 0; i < p.tiles_m; ++i) per += i / nb + 1;
-  }
-  const int nunits = p.L * per;
-  set_smem(ns_gemm_kernel<BN, MODE>, ns_smem<BN>());
-  const unsigned grid = unsigned(std::min(nunits, 148));
-  launch_k(ns_gemm_kernel<BN, MODE>, grid, kNsThreads, ns_smem<BN>(), s, ah, al, bh, bl, p, nunits,
-           per);
+  p.tiles_m = (p.M + kNsTile - 1) / kNsTile;
+  const int tiles_n = (p.cols + kNsTile - 1) / kNsTile;
+  p.per = SYM ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * tiles_n;
+  p.nunits = p.L * p.per;
+  set_smem(ns_gemm_kernel<PROD, MODE>, ns_smem<PROD>());
+  const unsigned grid = 2 * unsigned(std::min(p.nunits, 74));
+  const NsEpiMaps em{c[0], c[1], d[0], d[1]};
+  launch_cluster_k(ns_gemm_kernel<PROD, MODE>, grid, ns_threads<PROD>(), 2, ns_smem<PROD>(), s, a[0],
+                   a[1], b[0], b[1], em, p);
 }
 
 }  // namespace cyfa
@@ -502,12 +735,12 @@ int cyfa_newton_schulz(const void* g, int dtype, int L, int m, int n, int steps,
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int tall = m > n;
   const long long per = (long long)m * n;
-  const int parts = int(std::min<long long>(kNsNormParts, (per + 4095) / 4096));
+  const int parts = int(std::min<long long>(kNsNormParts, (per + 16383) / 16384));
   if (dtype == 1)
-    CYFA_LAUNCH("ns_norm", s, (launch_k(ns_norm_kernel<__nv_bfloat16>, dim3(parts, L), 256, 0, s,
+    CYFA_LAUNCH("ns_norm", s, (launch_k(ns_norm_kernel<__nv_bfloat16>, dim3(parts, L), kNsNormThreads, 0, s,
                                         static_cast<const __nv_bfloat16*>(g), per, w.part)));
   else
-    CYFA_LAUNCH("ns_norm", s, (launch_k(ns_norm_kernel<float>, dim3(parts, L), 256, 0, s,
+    CYFA_LAUNCH("ns_norm", s, (launch_k(ns_norm_kernel<float>, dim3(parts, L), kNsNormThreads, 0, s,
                                         static_cast<const float*>(g), per, w.part)));
   __nv_bfloat16* o = static_cast<__nv_bfloat16*>(out);
   if (steps == 0) {
@@ -522,7 +755,7 @@ int cyfa_newton_schulz(const void* g, int dtype, int L, int m, int n, int steps,
     return launch_status();
   }
   {
-    const dim3 grid(unsigned((n + 31) / 32), unsigned((m + 31) / 32), unsigned(L));
+    const dim3 grid(unsigned((n + 63) / 64), unsigned((m + 63) / 64), unsigned(L));
     if (dtype == 1)
       CYFA_LAUNCH("ns_split", s, (launch_k(ns_split_kernel<__nv_bfloat16>, grid, 256, 0, s,
                                            static_cast<const __nv_bfloat16*>(g), m, n, w.part, parts,
@@ -532,54 +765,56 @@ int cyfa_newton_schulz(const void* g, int dtype, int L, int m, int n, int steps,
                                            static_cast<const float*>(g), m, n, w.part, parts, eps,
                                            w.xh[0], w.xl[0], w.ldx, tall)));
   }
-  constexpr int BN = 256;
-  CUtensorMap xa[2][2], xb[2][2], xk[2][2], aa[2], ab[2], ba[2];
-  for (int i = 0; i < 2; ++i)
-    for (int h = 0; h < 2; ++h) {
-      const __half* x = h ? w.xl[i] : w.xh[i];
-      int rc = ns_tmap(&xa[i][h], x, L, w.M, w.N, w.ldx, 128);
-      if (!rc) rc = ns_tmap(&xb[i][h], x, L, w.M, w.N, w.ldx, BN);
-      if (!rc) rc = ns_tmap(&xk[i][h], x, L, w.M, w.N, w.ldx, 64);
-      if (rc) return rc;
-    }
+  // rows x 64 columns of X, A and B for the operands read along their rows, 64 x 64
+  // of X for B X, where X is read down its columns
+  // and 32 x 32 blocks for the finishing warps
+  CUtensorMap xa[2][2], xk[2][2], xe[2][2], aa[2], ba[2], ae[2], be[2];
   for (int h = 0; h < 2; ++h) {
-    int rc = ns_tmap(&aa[h], h ? w.al : w.ah, L, w.M, w.M, w.lda, 128);
-    if (!rc) rc = ns_tmap(&ab[h], h ? w.al : w.ah, L, w.M, w.M, w.lda, BN);
-    if (!rc) rc = ns_tmap(&ba[h], h ? w.bl : w.bh, L, w.M, w.M, w.lda, 128);
+    int rc = kOk;
+    for (int i = 0; i < 2 && !rc; ++i) {
+      const __half* x = h ? w.xl[i] : w.xh[i];
+      rc = ns_tmap(&xa[i][h], x, L, w.M, w.N, w.ldx, 64, 128);
+      if (!rc) rc = ns_tmap(&xk[i][h], x, L, w.M, w.N, w.ldx, 64, 64);
+      if (!rc) rc = ns_tmap(&xe[i][h], x, L, w.M, w.N, w.ldx, 32, 32);
+    }
+    const __half *a_ = h ? w.al : w.ah, *b_ = h ? w.bl : w.bh;
+    if (!rc) rc = ns_tmap(&aa[h], a_, L, w.M, w.M, w.lda, 64, 128);
+    if (!rc) rc = ns_tmap(&ae[h], a_, L, w.M, w.M, w.lda, 32, 32);
+    if (!rc) rc = ns_tmap(&ba[h], b_, L, w.M, w.M, w.lda, 64, 128);
+    if (!rc) rc = ns_tmap(&be[h], b_, L, w.M, w.M, w.lda, 32, 32);
     if (rc) return rc;
   }
   for (int step = 0; step < steps; ++step) {
     const int i = step & 1, last = step == steps - 1;
+    // matrices of one tile row: rounding errors average over few entries, and the
+    // time is the launches' latency
+    const bool all = w.M <= kNsTile, full = all || steps - step <= kNsFullSteps;
     NsGemmParams p{};
     p.L = L;
     p.M = w.M;
     p.out = o;
     p.tall = tall;
     p.cols = w.M;
-    p.ld = w.lda;
     p.K = w.N;
-    p.dh = w.ah;
-    p.dl = w.al;
-    CYFA_LAUNCH("ns_gram", s, (ns_launch<BN, kNsGram>(xa[i][0], xa[i][1], xb[i][0], xb[i][1], p, s)));
+    if (all)
+      CYFA_LAUNCH("ns_gram", s, (ns_launch<3, kNsGram>(xa[i], xa[i], ae, ae, p, s)));
+    else
+      CYFA_LAUNCH("ns_gram_1", s, (ns_launch<1, kNsGram>(xa[i], xa[i], ae, ae, p, s)));
     p.K = w.M;
     p.alpha = c;
     p.beta = b;
-    p.ch = w.ah;
-    p.cl = w.al;
-    p.dh = w.bh;
-    p.dl = w.bl;
-    CYFA_LAUNCH("ns_poly", s, (ns_launch<BN, kNsPoly>(aa[0], aa[1], ab[0], ab[1], p, s)));
-    p.cols = w.N;
-    p.ld = w.ldx;
-    p.beta = a;
-    p.ch = w.xh[i];
-    p.cl = w.xl[i];
-    p.dh = w.xh[1 - i];
-    p.dl = w.xl[1 - i];
-    if (last)
-      CYFA_LAUNCH("ns_last", s, (ns_launch<BN, kNsLast>(ba[0], ba[1], xk[i][0], xk[i][1], p, s)));
+    if (full)
+      CYFA_LAUNCH("ns_poly", s, (ns_launch<3, kNsPoly>(aa, aa, ae, be, p, s)));
     else
-      CYFA_LAUNCH("ns_step", s, (ns_launch<BN, kNsStep>(ba[0], ba[1], xk[i][0], xk[i][1], p, s)));
+      CYFA_LAUNCH("ns_poly_1", s, (ns_launch<1, kNsPoly>(aa, aa, ae, be, p, s)));
+    p.cols = w.N;
+    p.beta = a;
+    if (last)
+      CYFA_LAUNCH("ns_last", s, (ns_launch<3, kNsLast>(ba, xk[i], xe[i], xe[i], p, s)));
+    else if (full)
+      CYFA_LAUNCH("ns_step", s, (ns_launch<3, kNsStep>(ba, xk[i], xe[i], xe[1 - i], p, s)));
+    else
+      CYFA_LAUNCH("ns_step_1", s, (ns_launch<1, kNsStep>(ba, xk[i], xe[i], xe[1 - i], p, s)));
   }
   return launch_status();
 }

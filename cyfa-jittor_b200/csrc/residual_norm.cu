@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(1024) residual_norm_fwd_kernel(ResNormParams p
       R::load_f32(p.post, D, w);
 #pragma unroll
       for (int i = 0; i < kRnElems; ++i) z[i] = z[i] * rs * w[i];
-      if (in && threadIdx.x == 0) p.rstd_y[row] = rs;
+      if (in && threadIdx.x == 0 && p.rstd_y) p.rstd_y[row] = rs;
     }
     if (p.gate) {
       float g[kRnElems];
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(1024) residual_norm_fwd_kernel(ResNormParams p
 #pragma unroll
   for (int i = 0; i < kRnElems; ++i) ss = fmaf(t[i], t[i], ss);
   const float rs = rsqrtf(row_sum(ss, red) / p.D + p.eps);
-  if (in && threadIdx.x == 0) p.rstd_x[row] = rs;
+  if (in && threadIdx.x == 0 && p.rstd_x) p.rstd_x[row] = rs;
   float w[kRnElems];
   R::load_f32(p.weight, D, w);
 #pragma unroll
@@ -333,8 +333,8 @@ extern "C" {
 
 int cyfa_residual_norm_fwd(const cyfa_residual_norm_args* a, void* xn, void* h, float* rstd_x,
                            float* rstd_y, void* stream) {
-  CYFA_REQUIRE(a && a->x && a->weight && h && rstd_x && (!a->y || xn) &&
-                   (!a->post_weight || (a->y && rstd_y)) && (!a->gate || a->y),
+  CYFA_REQUIRE(a && a->x && a->weight && h && (!a->y || xn) &&
+                   (!a->post_weight || a->y) && (!a->gate || a->y),
                kNullPointer);
   const int rc = rn_checks(a->dtype, a->rows, a->D);
   if (rc) return rc;

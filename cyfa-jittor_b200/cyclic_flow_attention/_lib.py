@@ -182,6 +182,12 @@ def stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def raw_stream():
+    """The current stream of the current device as an int, for per-call paths that
+    hold CUDA tensors already (a fraction of a microsecond; ``stream()`` takes 3)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
 @contextlib.contextmanager
 def deferred(aux):
     """Inside the block, the library's final parameter-gradient reductions run on

@@ -18,19 +18,21 @@ def dtype_code(name, t):
     return code
 
 
-def same_device(**tensors):
-    """Raises unless all tensors are CUDA tensors of one device."""
-    _lib.require_cuda(*tensors.values())
-    devices = {n: t.device for n, t in tensors.items() if t is not None}
-    if len(set(devices.values())) > 1:
-        raise ValueError("tensors must be on one device, got "
-                         + ", ".join(f"{n} on {d}" for n, d in devices.items()))
+def same_device(first, *others):
+    """Raises unless `first` and the given others are CUDA tensors of one device."""
+    device = first.device
+    for t in others:
+        if t is not None and t.device != device:
+            _lib.require_cuda(first, t)
+            raise ValueError(f"tensors must be on one device, got {device} and {t.device}")
+    if device.type != "cuda":
+        _lib.require_cuda(first)
 
 
 def on_device(t):
     """Makes t's device the current one (the library launches on the current
     device and on its current stream)."""
-    if t.device.index == torch.cuda.current_device():
+    if t.device.index == torch._C._cuda_getDevice():
         return _NO_GUARD
     return torch.cuda.device(t.device)
 
@@ -38,7 +40,11 @@ def on_device(t):
 def row_levels(x, most):
     """The leading dimensions of x as at most `most` (size, stride) levels,
     outermost first, when its last dimension is dense; None if they need more."""
-    if x.shape[-1] > 1 and x.stride(-1) != 1:
+    width = x.shape[-1]
+    if x.is_contiguous():
+        rows = x.numel() // width
+        return [(rows, width)] if rows > 1 else []
+    if width > 1 and x.stride(-1) != 1:
         return None
     levels = []
     for size, stride in zip(x.shape[:-1], x.stride()[:-1]):
@@ -54,12 +60,21 @@ def row_levels(x, most):
 def as_rows(x):
     """(x, row stride) with x's leading dimensions one evenly spaced run of rows;
     x is copied if they are not."""
+    if x.is_contiguous():
+        return x, x.shape[-1]
     levels = row_levels(x, 1)
     if levels is None:
         x = x.contiguous()
-        levels = row_levels(x, 1)
+        return x, x.shape[-1]
     return x, (levels[0][1] if levels else x.shape[-1])
 
 
 def f32(t):
-    return None if t is None else t.detach().to(torch.float32).contiguous()
+    """A dense fp32 tensor with t's values (t itself when it is one)."""
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.detach().to(torch.float32).contiguous()
+
+
+def address(t):
+    return None if t is None else t.data_ptr()

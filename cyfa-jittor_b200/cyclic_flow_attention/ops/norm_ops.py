@@ -13,7 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._rows import as_rows, dtype_code, f32, on_device, same_device
+from ._rows import address, as_rows, dtype_code, f32, on_device, same_device
 
 MAX_WIDTH = 8192
 
@@ -27,26 +27,25 @@ def _args(x, y, gate, weight, post, scale_vector, scale, eps):
         y, sy = as_rows(y)
     if gate is not None:
         gate, sg = as_rows(gate)
-    p = lambda t: None if t is None else t.data_ptr()
+    p = address
     return _lib.ResidualNormArgs(
         x.numel() // D, D, dtype_code("x", x), p(x), p(y), p(gate), sx, sy, sg, p(weight),
         p(post), p(scale_vector), scale, eps), (x, y, gate)
 
 
-def _forward(x, y, weight, post, gate, scale_vector, scale, eps):
-    """(xn or None, h, rstd_x, rstd_y)."""
+def _forward(x, y, weight, post, gate, scale_vector, scale, eps, keep):
+    """(xn or None, h, rstd_x, rstd_y); the last two, which only the backward
+    reads, are None unless `keep`."""
     rows = x.numel() // x.shape[-1]
-    dev = x.device
-    xn = None if y is None else torch.empty(x.shape, device=dev, dtype=x.dtype)
-    h = torch.empty(x.shape, device=dev, dtype=x.dtype)
-    rstd = torch.empty(2 if post is not None else 1, rows, device=dev, dtype=torch.float32)
-    rstd_x = rstd[0]
-    rstd_y = rstd[1] if post is not None else None
+    xn = None if y is None else x.new_empty(x.shape)
+    h = x.new_empty(x.shape)
+    rstd_x = weight.new_empty(rows) if keep else None
+    rstd_y = weight.new_empty(rows) if keep and post is not None else None
     if rows:
         args, _keep = _args(x, y, gate, weight, post, scale_vector, scale, eps)
         with on_device(x):
-            _lib.call("cyfa_residual_norm_fwd", ctypes.byref(args), _lib.ptr(xn), h.data_ptr(),
-                      rstd_x.data_ptr(), _lib.ptr(rstd_y), _lib.stream())
+            _lib.call("cyfa_residual_norm_fwd", ctypes.byref(args), address(xn), h.data_ptr(),
+                      address(rstd_x), address(rstd_y), _lib.raw_stream())
     return xn, h, rstd_x, rstd_y
 
 
@@ -57,7 +56,7 @@ class ResidualNormFunction(torch.autograd.Function):
     def forward(ctx, x, y, weight, post, gate, scale_vector, scale, eps):
         ctx.set_materialize_grads(False)
         w, pw, sv = f32(weight), f32(post), f32(scale_vector)
-        xn, h, rstd_x, rstd_y = _forward(x, y, w, pw, gate, sv, scale, eps)
+        xn, h, rstd_x, rstd_y = _forward(x, y, w, pw, gate, sv, scale, eps, True)
         plain = post is None and gate is None and scale_vector is None and scale == 1.0
         # the plain sum needs y for no gradient
         ctx.save_for_backward(x if xn is None else xn, None if plain else y, w, pw, gate, sv,
@@ -81,9 +80,8 @@ class ResidualNormFunction(torch.autograd.Function):
         dh = None if dh is None else dh.to(t.dtype).contiguous()
         full = has_y and not plain
         want_x = need[0] or (plain and has_y and need[1])
-        rowwise = lambda on: torch.empty(t.shape, device=dev, dtype=t.dtype) if on else None
-        column = lambda on: torch.zeros(D, device=dev, dtype=torch.float32) if on and not rows \
-            else (torch.empty(D, device=dev, dtype=torch.float32) if on else None)
+        rowwise = lambda on: t.new_empty(t.shape) if on else None
+        column = lambda on: (w.new_empty(D) if rows else w.new_zeros(D)) if on else None
         dx = rowwise(want_x)
         dy = rowwise(full and need[1])
         dgate = rowwise(gate is not None and need[4])
@@ -94,11 +92,11 @@ class ResidualNormFunction(torch.autograd.Function):
             args, _keep = _args(t, y if full else None, gate, w, pw, sv, scale, eps)
             nbytes = _lib.lib().cyfa_residual_norm_bwd_work_bytes(rows, D)
             work = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-            P = _lib.ptr
+            P = address
             with on_device(t):
                 _lib.call("cyfa_residual_norm_bwd", ctypes.byref(args), rstd_x.data_ptr(),
                           P(rstd_y), P(dxn), P(dh), P(dx), P(dy), P(dgate), P(dw), P(dpost),
-                          P(dscale), work.data_ptr(), ctypes.c_size_t(nbytes), _lib.stream())
+                          P(dscale), work.data_ptr(), nbytes, _lib.raw_stream())
         if plain and has_y and need[1]:
             dy = dx
         dw, dpost, dscale = (g if g is None else g.to(d)
@@ -142,12 +140,11 @@ def residual_norm(x, y, weight, post_weight=None, gate=None, scale=None, eps=1e-
     number = 1.0 if scale is None or scale_vector is not None else float(scale)
     if not (math.isfinite(number) and math.isfinite(eps) and eps >= 0):
         raise ValueError(f"scale and eps must be finite and eps >= 0, got {scale}, {eps}")
-    same_device(x=x, y=y, weight=weight, post_weight=post_weight, gate=gate, scale=scale_vector)
+    same_device(x, y, weight, post_weight, gate, scale_vector)
     tensors = (x, y, weight, post_weight, gate, scale_vector)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         out = ResidualNormFunction.apply(*tensors, number, float(eps))
         return (x, out[0]) if y is None else out
-    xn, h, _, _ = _forward(x.detach(), None if y is None else y.detach(), f32(weight),
-                           f32(post_weight), None if gate is None else gate.detach(),
-                           f32(scale_vector), number, float(eps))
+    xn, h, _, _ = _forward(x, y, f32(weight), f32(post_weight), gate, f32(scale_vector), number,
+                           float(eps), False)
     return x if xn is None else xn, h

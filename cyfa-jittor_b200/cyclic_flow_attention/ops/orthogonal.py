@@ -4,7 +4,6 @@ The counterpart for matrices of the element-wise AdamW update (the reference's
 only optimizer, training/optim.py:8-124); ``training.optim.Muon`` applies it.
 """
 
-import ctypes
 import math
 
 import torch
@@ -44,15 +43,15 @@ def orthogonalize(g, steps=5, coefficients=QUINTIC, eps=1e-7):
     L = math.prod(g.shape[:-2])
     if L > 65535:
         raise ValueError(f"at most 65535 matrices per call, got {L}")
-    same_device(g=g)
+    same_device(g)
     out = torch.empty(g.shape, device=g.device, dtype=torch.bfloat16)
     if out.numel() == 0:
         return out
-    x = g.detach().contiguous()
+    x = g.contiguous()
     nbytes = _lib.lib().cyfa_newton_schulz_work_bytes(L, m, n)
     work = torch.empty(nbytes, device=g.device, dtype=torch.uint8)
     with on_device(x):
         _lib.call("cyfa_newton_schulz", x.data_ptr(), code, L, m, n, int(steps),
                   *(float(c) for c in coefficients), float(eps), out.data_ptr(), work.data_ptr(),
-                  ctypes.c_size_t(nbytes), _lib.stream())
+                  nbytes, _lib.raw_stream())
     return out

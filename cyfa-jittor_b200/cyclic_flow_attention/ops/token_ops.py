@@ -8,7 +8,6 @@ direction is libcyfa kernels that read the logits, or the gradient rows, once an
 build no fp32 copy of them.
 """
 
-import ctypes
 import math
 from typing import NamedTuple, Optional
 
@@ -16,7 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._rows import dtype_code, on_device, row_levels, same_device
+from ._rows import address, dtype_code, f32, on_device, row_levels, same_device
 
 MAX_TOP = 32
 _INTS = (torch.int64, torch.int32)
@@ -29,6 +28,12 @@ class TokenLogProbs(NamedTuple):
     entropy: torch.Tensor
     top_logp: Optional[torch.Tensor]
     top_tokens: Optional[torch.Tensor]
+
+
+def _dense_int64(tokens):
+    if tokens.dtype == torch.int64 and tokens.is_contiguous():
+        return tokens
+    return tokens.to(torch.int64).contiguous()
 
 
 def _addressed(logits):
@@ -45,25 +50,24 @@ def _addressed(logits):
     return logits, levels[1][0], levels[0][1], levels[1][1]
 
 
-def _logprobs_fwd(logits, tokens, top, ignore_index):
-    """(addressed logits, logp, entropy, stats, top_logp, top_tokens)."""
-    shape, V, dev = tokens.shape, logits.shape[-1], logits.device
+def _logprobs_fwd(logits, tokens, top, ignore_index, keep):
+    """(addressed logits, logp, entropy, stats, top_logp, top_tokens); stats, which
+    only the backward reads, is None unless `keep`."""
     rows = tokens.numel()
     x, inner, outer_stride, inner_stride = _addressed(logits)
-    f32 = torch.float32
-    logp = torch.empty(shape, device=dev, dtype=f32)
-    entropy = torch.empty(shape, device=dev, dtype=f32)
-    stats = torch.empty(rows, 2, device=dev, dtype=f32)
+    logp = torch.empty_like(tokens, dtype=torch.float32)
+    entropy = torch.empty_like(logp)
+    stats = logp.new_empty((rows, 2)) if keep else None
     top_logp = top_tokens = None
     if top:
-        top_logp = torch.empty(*shape, top, device=dev, dtype=f32)
-        top_tokens = torch.empty(*shape, top, device=dev, dtype=torch.int64)
+        top_logp = logp.new_empty((*tokens.shape, top))
+        top_tokens = tokens.new_empty((*tokens.shape, top))
     if rows:
         with on_device(x):
             _lib.call("cyfa_token_logprobs_fwd", x.data_ptr(), dtype_code("logits", x), rows,
-                      inner, outer_stride, inner_stride, V, tokens.data_ptr(), ignore_index, top,
-                      logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(), _lib.ptr(top_logp),
-                      _lib.ptr(top_tokens), _lib.stream())
+                      inner, outer_stride, inner_stride, x.shape[-1], tokens.data_ptr(),
+                      ignore_index, top, logp.data_ptr(), entropy.data_ptr(), address(stats),
+                      address(top_logp), address(top_tokens), _lib.raw_stream())
     return x, logp, entropy, stats, top_logp, top_tokens
 
 
@@ -74,7 +78,7 @@ class TokenLogProbsFunction(torch.autograd.Function):
     def forward(ctx, logits, tokens, top, ignore_index):
         ctx.set_materialize_grads(False)
         x, logp, entropy, stats, top_logp, top_tokens = _logprobs_fwd(logits, tokens, top,
-                                                                     ignore_index)
+                                                                     ignore_index, True)
         ctx.save_for_backward(x, tokens, stats, entropy)
         ctx.ignore_index = ignore_index
         if not top:
@@ -89,16 +93,15 @@ class TokenLogProbsFunction(torch.autograd.Function):
             return None, None, None, None
         x, tokens, stats, entropy = ctx.saved_tensors
         x, inner, outer_stride, inner_stride = _addressed(x)
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        dx = x.new_empty(x.shape)
         rows = tokens.numel()
-        dlogp = None if dlogp is None else dlogp.float().contiguous()
-        dentropy = None if dentropy is None else dentropy.float().contiguous()
+        dlogp, dentropy = f32(dlogp), f32(dentropy)
         if rows:
             with on_device(x):
                 _lib.call("cyfa_token_logprobs_bwd", x.data_ptr(), dtype_code("logits", x), rows,
                           inner, outer_stride, inner_stride, x.shape[-1], tokens.data_ptr(),
                           ctx.ignore_index, stats.data_ptr(), entropy.data_ptr(),
-                          _lib.ptr(dlogp), _lib.ptr(dentropy), dx.data_ptr(), _lib.stream())
+                          address(dlogp), address(dentropy), dx.data_ptr(), _lib.raw_stream())
         return dx, None, None, None
 
 
@@ -133,25 +136,25 @@ def token_log_probs(logits, tokens, top=0, ignore_index=-100):
         raise ValueError(f"top must be between 0 and {min(MAX_TOP, V)}, got {top}")
     if tokens.numel() >= 1 << 27:
         raise ValueError(f"{tokens.numel()} positions; at most {(1 << 27) - 1} per call")
-    same_device(logits=logits, tokens=tokens)
+    same_device(logits, tokens)
     top, ignore_index = int(top), int(ignore_index)
-    tokens = tokens.detach().to(torch.int64).contiguous()
+    tokens = _dense_int64(tokens)
     if torch.is_grad_enabled() and logits.requires_grad:
         out = TokenLogProbsFunction.apply(logits, tokens, top, ignore_index)
         return TokenLogProbs(*out, *((None, None) if not top else ()))
-    _, logp, entropy, _, top_logp, top_tokens = _logprobs_fwd(logits.detach(), tokens, top,
-                                                              ignore_index)
+    _, logp, entropy, _, top_logp, top_tokens = _logprobs_fwd(logits, tokens, top, ignore_index,
+                                                              False)
     return TokenLogProbs(logp, entropy, top_logp, top_tokens)
 
 
 def _embed_fwd(tokens, weight, scale):
     V, D = weight.shape
-    out = torch.empty(*tokens.shape, D, device=weight.device, dtype=weight.dtype)
+    out = weight.new_empty((*tokens.shape, D))
     if out.numel():
         with on_device(weight):
             _lib.call("cyfa_embed_fwd", tokens.data_ptr(), weight.data_ptr(),
                       dtype_code("weight", weight), out.data_ptr(), tokens.numel(), V, D, scale,
-                      _lib.stream())
+                      _lib.raw_stream())
     return out
 
 
@@ -163,7 +166,7 @@ class EmbedTokensFunction(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(tokens)
         ctx.meta = (weight.shape, weight.dtype, scale, padding_idx)
-        return _embed_fwd(tokens, weight.detach().contiguous(), scale)
+        return _embed_fwd(tokens, weight.contiguous(), scale)
 
     @staticmethod
     @once_differentiable
@@ -176,13 +179,13 @@ class EmbedTokensFunction(torch.autograd.Function):
         if N == 0:
             return None, torch.zeros(V, D, device=tokens.device, dtype=dtype), None, None
         dout = dout.to(dtype).contiguous()
-        dw = torch.empty(V, D, device=tokens.device, dtype=dtype)
+        dw = dout.new_empty((V, D))
         nbytes = _lib.lib().cyfa_embed_bwd_work_bytes(N, D)
         work = torch.empty(nbytes, device=tokens.device, dtype=torch.uint8)
         with on_device(dout):
             _lib.call("cyfa_embed_bwd", tokens.data_ptr(), dout.data_ptr(),
                       dtype_code("weight", dw), dw.data_ptr(), N, V, D, scale, padding_idx,
-                      work.data_ptr(), ctypes.c_size_t(nbytes), _lib.stream())
+                      work.data_ptr(), nbytes, _lib.raw_stream())
         return None, dw, None, None
 
 
@@ -212,8 +215,8 @@ def embed_tokens(tokens, weight, scale=1.0, padding_idx=None):
         if not -V <= padding_idx < V:
             raise ValueError(f"padding_idx {padding_idx} is outside a vocabulary of {V}")
         pad = int(padding_idx) % V
-    same_device(tokens=tokens, weight=weight)
-    tokens = tokens.detach().to(torch.int64).contiguous()
+    same_device(weight, tokens)
+    tokens = _dense_int64(tokens)
     if torch.is_grad_enabled() and weight.requires_grad:
         return EmbedTokensFunction.apply(tokens, weight, float(scale), pad)
-    return _embed_fwd(tokens, weight.detach().contiguous(), float(scale))
+    return _embed_fwd(tokens, weight.contiguous(), float(scale))

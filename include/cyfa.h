@@ -435,7 +435,7 @@ int cyfa_swiglu(const void* gu, void* out, int rows, int mid, void* stream);
  * logp 0 and no gradient from it; any other token outside [0, V) gives NaN, no
  * gradient and device error 3.  Masked logits (-inf) have probability 0; a row with
  * no finite logit has logp -inf, entropy 0 and zero gradient.
- * stats [rows, 2] f32 (row maximum, log of the sum) is kept for the backward;
+ * stats [rows, 2] f32 (row maximum, log of the sum) is kept for the backward (NULL without one);
  * top_logp / top_tokens [rows, top] may be NULL when top is 0. */
 int cyfa_token_logprobs_fwd(const void* logits, int dtype, long long rows, long long inner,
                             long long stride_outer, long long stride_inner, int V,
@@ -492,7 +492,7 @@ typedef struct {
 } cyfa_residual_norm_args;
 
 /* xn, h [rows, D] contiguous; rstd_x, rstd_y [rows] f32 kept for the backward
- * (rstd_y only with post_weight). */
+ * (either may be NULL without one; rstd_y only with post_weight). */
 int cyfa_residual_norm_fwd(const cyfa_residual_norm_args* args, void* xn, void* h, float* rstd_x,
                            float* rstd_y, void* stream);
 

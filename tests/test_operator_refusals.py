@@ -117,7 +117,7 @@ def test_c_refusals():
         a = _lib.ResidualNormArgs(rows, D, dtype, x, y, gate, D, D, D, ok, post, None, 1.0, 1e-6)
         return L.cyfa_residual_norm_fwd(ctypes.byref(a), xn, ok, ok, rstd_y, None)
 
-    assert rn(x=None) == 2 and rn(xn=None) == 2 and rn(post=ok) == 2 and rn(y=None, gate=ok) == 2
+    assert rn(x=None) == 2 and rn(xn=None) == 2 and rn(y=None, post=ok) == 2 and rn(y=None, gate=ok) == 2
     assert rn(D=8193) == 1 and rn(rows=0) == 1 and rn(dtype=5) == 4 and rn(x=odd) == 3
     a = _lib.ResidualNormArgs(2, 8, 1, ok, ok, None, 8, 8, 8, ok, None, None, 1.0, 1e-6)
     n = L.cyfa_residual_norm_bwd_work_bytes(2, 8)
