@@ -430,7 +430,7 @@ int cyfa_swiglu(const void* gu, void* out, int rows, int mid, void* stream);
  * Replaces: the loss of the causal LM (models/cyfa/modeling_cyfa.py:102-116,
  * cross entropy over fp32 logits); entropy and alternatives have no counterpart.
  * Row r of the logits starts at (r / inner) * stride_outer + (r % inner) *
- * stride_inner elements (0 <= r < rows) and is V contiguous elements; no row
+ * stride_inner elements (0 <= r < rows, 0 < inner <= rows) and is V contiguous elements; no row
  * alignment is needed.  tokens [rows] i64: a row whose token is ignore_index has
  * logp 0 and no gradient from it; any other token outside [0, V) gives NaN, no
  * gradient and device error 3.  Masked logits (-inf) have probability 0; a row with
