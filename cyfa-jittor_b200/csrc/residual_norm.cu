@@ -8,17 +8,15 @@
 //   dgate = dt scale z sigmoid(gate) (1 - sigmoid(gate)),  dscale = sum dt sigmoid(gate) z
 //   dy    = dz    or  (dz post - y^ mean(dz post y^)) / rms(y)
 //   dweight = sum dh x^,   dpost = sum dz y^   (over the rows)
-// All arithmetic is fp32.  Each thread owns 8 columns of a row (kept in
-// registers between the reductions and the stores), so every tensor is read and
-// written once; column sums go through per-CTA partial rows added in a fixed
-// order.
+// All arithmetic is fp32.  Each thread owns E columns of a row (kept in registers
+// between the reductions and the stores), so every tensor is read and written
+// once; column sums go through per-CTA partial rows added in a fixed order.
 #include <algorithm>
 
 #include "cyfa_common.cuh"
 
 namespace cyfa {
 
-constexpr int kRnElems = 8;        // columns of a thread
 constexpr int kRnMaxWidth = 8192;  // 1024 threads
 
 struct ResNormParams {
@@ -36,44 +34,41 @@ struct ResNormParams {
   const void *dxn, *dh;              // [rows, D] contiguous, may be null
   void *dx, *dy, *dgate;             // [rows, D] contiguous, may be null
   float* part;                       // [CTAs][3][D] column sums: dweight, dpost, dscale
+  int stages;                        // shared-memory slots of a streamed row: 2, or 1 (no copy ahead)
 };
 
-// The 8 columns of thread t among n threads: VEC consecutive ones at
-// (t + j n) VEC for j < 8 / VEC.
-template <typename T, int VEC>
+// A thread's 8 columns threadIdx.x + j blockDim.x of a row, for single elements.
+template <typename T>
 struct RnRow {
-  static constexpr int J = kRnElems / VEC;
-  static __device__ __forceinline__ int col(int j) {
-    return (int(threadIdx.x) + j * int(blockDim.x)) * VEC;
-  }
-  static __device__ __forceinline__ void load(const void* base, long long off, int D, float* f) {
-    const T* p = static_cast<const T*>(base) + off;
+  static constexpr int E = 8;
+  int off[E];
+  uint32_t mask;  // columns inside the row
+  __device__ __forceinline__ explicit RnRow(int D) : mask(0) {
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int c = col(j);
-      if (c < D) {
-        EmbVec<T, VEC>::load(p + c, f + j * VEC);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) f[j * VEC + i] = 0.f;
-      }
+    for (int j = 0; j < E; ++j) {
+      off[j] = int(threadIdx.x) + j * int(blockDim.x);
+      if (off[j] < D) mask |= 1u << j;
     }
   }
-  static __device__ __forceinline__ void load_f32(const float* p, int D, float* f) {
+  // p: the row, or null for zeros
+  __device__ __forceinline__ void load(const T* p, uint32_t m, float (&f)[E]) const {
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int c = col(j);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) f[j * VEC + i] = c < D ? __ldg(p + c + i) : 0.f;
-    }
+    for (int j = 0; j < E; ++j) f[j] = p && ((m >> j) & 1) ? float(p[off[j]]) : 0.f;
   }
-  static __device__ __forceinline__ void store(void* base, long long off, int D, const float* f) {
-    T* p = static_cast<T*>(base) + off;
+  __device__ __forceinline__ void param(const float* p, float (&f)[E]) const {
 #pragma unroll
-    for (int j = 0; j < J; ++j)
-      if (col(j) < D) EmbVec<T, VEC>::store(p + col(j), f + j * VEC);
+    for (int j = 0; j < E; ++j) f[j] = (mask >> j) & 1 ? __ldg(p + off[j]) : 0.f;
+  }
+  __device__ __forceinline__ void store(T* p, uint32_t m, const float (&f)[E]) const {
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if ((m >> j) & 1) p[off[j]] = T(f[j]);
   }
 };
+template <typename T>
+__device__ __forceinline__ const T* rn_at(const void* base, long long off) {
+  return base ? static_cast<const T*>(base) + off : nullptr;
+}
 
 // Sum over the threads of one row (threadIdx.x), the same in all of them and in
 // the same order.  red: one float per warp of the CTA.
@@ -91,182 +86,469 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   return s;
 }
 
-__device__ __forceinline__ float rn_sigmoid(float z) { return 1.f / (1.f + __expf(-z)); }
-
 template <typename T>
 __device__ __forceinline__ float rn_round(float v) {
   return float(T(v));
 }
 
-// blockDim (threads of a row, rows of a CTA)
-template <typename T, int VEC>
-__global__ void __launch_bounds__(1024) residual_norm_fwd_kernel(ResNormParams p) {
-  using R = RnRow<T, VEC>;
+// ------------------------------------------------ rows of 16-byte vectors
+// Persistent CTAs of blockDim (threads of a row, rows at a time).  Each thread copies
+// its E columns of the next row into its own shared-memory slots (cp.async, no
+// barrier: nobody else reads them) while it works on the current one, so that the
+// loads never wait for a row's sums and cost no registers.
+template <typename T, int E>
+struct RnStream {
+  static constexpr int VEC = 16 / sizeof(T), J = E / VEC;
+  uint32_t slot;     // shared address of the thread's first chunk
+  int threads, tensors;
+  int c0, cs;        // columns c0 + j cs ..
+  uint32_t mask;     // chunks inside the row
+  __device__ __forceinline__ RnStream(void* smem, int tensors_, int D)
+      : threads(int(blockDim.x * blockDim.y)), tensors(tensors_), c0(int(threadIdx.x) * VEC),
+        cs(int(blockDim.x) * VEC), mask(0) {
+    slot = smem_u32(smem) + (threadIdx.y * blockDim.x + threadIdx.x) * 16;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      if (c0 + j * cs < D) mask |= 1u << j;
+  }
+  __device__ __forceinline__ uint32_t at(int stage, int tensor, int j) const {
+    return slot + ((stage * tensors + tensor) * J + j) * threads * 16;
+  }
+  // row: at this thread's first column, or null for zeros
+  __device__ __forceinline__ void copy(int stage, int tensor, const T* row, uint32_t m) const {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const bool ok = row && ((m >> j) & 1);
+      cp_async16(at(stage, tensor, j), ok ? row + j * cs : row, ok);
+    }
+  }
+  __device__ __forceinline__ void get(int stage, int tensor, int j, float* f) const {
+    LpVec<T>::unpack(ld_shared_v4(at(stage, tensor, j)), f);
+  }
+  __device__ __forceinline__ void param(const float* p, int j, float* f) const {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4) {
+      const float4 v = (mask >> j) & 1 ? __ldg(reinterpret_cast<const float4*>(p + c0 + j * cs + i))
+                                       : make_float4(0.f, 0.f, 0.f, 0.f);
+      f[i] = v.x;
+      f[i + 1] = v.y;
+      f[i + 2] = v.z;
+      f[i + 3] = v.w;
+    }
+  }
+  static __device__ __forceinline__ void store(T* p, const uint4& u) {
+    *reinterpret_cast<uint4*>(p) = u;
+  }
+};
+
+// PLAIN: y alone, no post-norm, gate or scale.
+template <typename T, int E, bool PLAIN>
+__global__ void __launch_bounds__(256) residual_norm_fwd_stream_kernel(ResNormParams p) {
+  using S = RnStream<T, E>;
+  constexpr int VEC = S::VEC, J = S::J;
+  extern __shared__ __align__(16) uint8_t rn_smem[];
+  __shared__ float red[32];
   pdl_wait();
   pdl_trigger();
-  __shared__ float red[32];
-  const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
-  const bool in = row < p.rows;
-  const int D = in ? p.D : 0;  // rows past the end take part in the barriers only
-  float t[kRnElems];
-  R::load(p.x, row * p.sx, D, t);
-  if (p.y) {
-    float z[kRnElems];
-    R::load(p.y, row * p.sy, D, z);
-    if (p.post) {
+  const int D = p.D;
+  const S st(rn_smem, PLAIN ? 2 : 1 + (p.y != nullptr) + (p.gate != nullptr), D);
+  const long long step = (long long)gridDim.x * blockDim.y;
+  auto fetch = [&](long long row, int stage) {
+    const uint32_t m = row < p.rows ? st.mask : 0;
+    st.copy(stage, 0, rn_at<T>(p.x, row * p.sx + st.c0), m);
+    if (PLAIN || p.y) st.copy(stage, 1, rn_at<T>(p.y, row * p.sy + st.c0), m);
+    if (!PLAIN && p.gate) st.copy(stage, 2, rn_at<T>(p.gate, row * p.sgate + st.c0), m);
+    cp_async_commit();
+  };
+  long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+  const int flip = p.stages - 1;
+  if (flip) fetch(row, 0);
+  for (int s = 0; row - threadIdx.y < p.rows; row += step, s ^= flip) {
+    fetch(flip ? row + step : row, s ^ flip);
+    if (flip) cp_async_wait<1>(); else cp_async_wait<0>();
+    const uint32_t m = row < p.rows ? st.mask : 0;
+    const bool first = row < p.rows && threadIdx.x == 0;
+    T* xn = static_cast<T*>(p.xn) + row * D + st.c0;
+    T* h = static_cast<T*>(p.h) + row * D + st.c0;
+    float rsy = 1.f;
+    if (!PLAIN && p.post) {
       float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < kRnElems; ++i) ss = fmaf(z[i], z[i], ss);
-      const float rs = rsqrtf(row_sum(ss, red) / p.D + p.eps);
-      float w[kRnElems];
-      R::load_f32(p.post, D, w);
+      for (int j = 0; j < J; ++j) {
+        float y[VEC];
+        st.get(s, 1, j, y);
 #pragma unroll
-      for (int i = 0; i < kRnElems; ++i) z[i] = z[i] * rs * w[i];
-      if (in && threadIdx.x == 0 && p.rstd_y) p.rstd_y[row] = rs;
+        for (int i = 0; i < VEC; ++i) ss = fmaf(y[i], y[i], ss);
+      }
+      rsy = rsqrtf(row_sum(ss, red) / D + p.eps);
+      if (first && p.rstd_y) p.rstd_y[row] = rsy;
     }
-    if (p.gate) {
-      float g[kRnElems];
-      R::load(p.gate, row * p.sgate, D, g);
+    float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < kRnElems; ++i) z[i] *= rn_sigmoid(g[i]);
+    for (int j = 0; j < J; ++j) {
+      float t[VEC];
+      st.get(s, 0, j, t);
+      if (PLAIN || p.y) {
+        float z[VEC];
+        st.get(s, 1, j, z);
+        if (!PLAIN) {
+          float f[VEC];
+          if (p.post) {
+            st.param(p.post, j, f);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) z[i] = z[i] * rsy * f[i];
+          }
+          if (p.gate) {
+            st.get(s, 2, j, f);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) z[i] *= sigmoid_mufu(f[i]);
+          }
+          if (p.scale_v) {
+            st.param(p.scale_v, j, f);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) z[i] *= f[i];
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) z[i] *= p.scale;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) t[i] += z[i];
+        // the norm reads the stream as it is kept, in x's type
+        const uint4 u = LpVec<T>::pack(t);
+        LpVec<T>::unpack(u, t);
+        st_shared_v4(st.at(s, 0, j), u.x, u.y, u.z, u.w);
+        if ((m >> j) & 1) S::store(xn + j * st.cs, u);
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) ss = fmaf(t[i], t[i], ss);
     }
-    if (p.scale_v) {
-      float s[kRnElems];
-      R::load_f32(p.scale_v, D, s);
+    const float rs = rsqrtf(row_sum(ss, red) / D + p.eps);
+    if (first && p.rstd_x) p.rstd_x[row] = rs;
 #pragma unroll
-      for (int i = 0; i < kRnElems; ++i) z[i] *= s[i];
-    } else {
+    for (int j = 0; j < J; ++j) {
+      float t[VEC], w[VEC];
+      st.get(s, 0, j, t);
+      st.param(p.weight, j, w);
 #pragma unroll
-      for (int i = 0; i < kRnElems; ++i) z[i] *= p.scale;
+      for (int i = 0; i < VEC; ++i) t[i] = t[i] * rs * w[i];
+      if ((m >> j) & 1) S::store(h + j * st.cs, LpVec<T>::pack(t));
     }
-    // the norm reads the stream as it is kept, in x's type
-#pragma unroll
-    for (int i = 0; i < kRnElems; ++i) t[i] = rn_round<T>(t[i] + z[i]);
-    R::store(p.xn, row * p.D, D, t);
   }
-  float ss = 0.f;
-#pragma unroll
-  for (int i = 0; i < kRnElems; ++i) ss = fmaf(t[i], t[i], ss);
-  const float rs = rsqrtf(row_sum(ss, red) / p.D + p.eps);
-  if (in && threadIdx.x == 0 && p.rstd_x) p.rstd_x[row] = rs;
-  float w[kRnElems];
-  R::load_f32(p.weight, D, w);
-#pragma unroll
-  for (int i = 0; i < kRnElems; ++i) t[i] = t[i] * rs * w[i];
-  R::store(p.h, row * p.D, D, t);
+  cp_async_wait<0>();
 }
 
-// p.x is the new stream x' here (contiguous or strided by sx).  A CTA walks its
-// rows with the column sums in registers.
-template <typename T, int VEC, bool FULL>
-__global__ void __launch_bounds__(1024) residual_norm_bwd_kernel(ResNormParams p) {
-  using R = RnRow<T, VEC>;
+// The column sums of a CTA's threads (dweight and, with FULL, dpost and dscale): its
+// row slots side by side in shared memory [rows][D], then added in order, as one
+// partial row.
+template <int SETS, typename Put>
+__device__ __forceinline__ void rn_partial(float* out, float* buf, int D, Put put) {
+  const int tid = int(threadIdx.y * blockDim.x + threadIdx.x), n = int(blockDim.x * blockDim.y);
+#pragma unroll
+  for (int k = 0; k < SETS; ++k) {
+    __syncthreads();
+    put(k, buf + threadIdx.y * D);
+    __syncthreads();
+    for (int c = tid; c < D; c += n) {
+      float v = buf[c];
+      for (int y = 1; y < int(blockDim.y); ++y) v += buf[y * D + c];
+      out[k * D + c] = v;
+    }
+  }
+}
+
+// p.x is the new stream x'.  FULL: with y's side; otherwise dx alone (the plain sum's
+// dy equals it).
+template <typename T, int E, bool FULL>
+__global__ void __launch_bounds__(256) residual_norm_bwd_stream_kernel(ResNormParams p) {
+  using S = RnStream<T, E>;
+  constexpr int VEC = S::VEC, J = S::J;
+  extern __shared__ __align__(16) uint8_t rn_smem[];
+  __shared__ float red[32];
+  pdl_wait();
+  pdl_trigger();
+  const int D = p.D;
+  const S st(rn_smem, FULL ? 4 + (p.gate != nullptr) : 3, D);
+  const float inv = 1.f / D;
+  const long long step = (long long)gridDim.x * blockDim.y;
+  auto fetch = [&](long long row, int stage) {
+    const uint32_t m = row < p.rows ? st.mask : 0;
+    st.copy(stage, 0, rn_at<T>(p.x, row * p.sx + st.c0), m);
+    st.copy(stage, 1, rn_at<T>(p.dh, row * D + st.c0), m);
+    st.copy(stage, 2, rn_at<T>(p.dxn, row * D + st.c0), m);
+    if (FULL) {
+      st.copy(stage, 3, rn_at<T>(p.y, row * p.sy + st.c0), m);
+      if (p.gate) st.copy(stage, 4, rn_at<T>(p.gate, row * p.sgate + st.c0), m);
+    }
+    cp_async_commit();
+  };
+  float acc[FULL ? 3 : 1][E];  // dweight, dpost, dscale
+#pragma unroll
+  for (int k = 0; k < (FULL ? 3 : 1); ++k)
+#pragma unroll
+    for (int i = 0; i < E; ++i) acc[k][i] = 0.f;
+  long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+  const int flip = p.stages - 1;
+  if (flip) fetch(row, 0);
+  for (int s = 0; row - threadIdx.y < p.rows; row += step, s ^= flip) {
+    fetch(flip ? row + step : row, s ^ flip);
+    const bool in = row < p.rows;
+    const uint32_t m = in ? st.mask : 0;
+    const float rs = in ? p.rstd_x[row] : 0.f;
+    const float rsy = FULL && p.post && in ? p.rstd_y[row] : 1.f;
+    if (flip) cp_async_wait<1>(); else cp_async_wait<0>();
+    float dot = 0.f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      float t[VEC], g[VEC], w[VEC];
+      st.get(s, 0, j, t);
+      st.get(s, 1, j, g);
+      st.param(p.weight, j, w);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float gt = g[i] * t[i];  // rs, the same for the row, comes in once below
+        acc[0][j * VEC + i] = fmaf(gt, rs, acc[0][j * VEC + i]);
+        dot = fmaf(gt, w[i], dot);
+      }
+    }
+    // dt = dxn + rs g w - t rs^2 dot
+    dot = row_sum(dot * rs, red) * inv * rs * rs;
+    float dz[FULL ? E : 1], doty = 0.f;
+    T* dx = static_cast<T*>(p.dx) + row * D + st.c0;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      float t[VEC], g[VEC], dt[VEC], w[VEC];
+      st.get(s, 0, j, t);
+      st.get(s, 1, j, g);
+      st.get(s, 2, j, dt);
+      st.param(p.weight, j, w);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) dt[i] = fmaf(g[i] * w[i], rs, fmaf(-dot, t[i], dt[i]));
+      if (p.dx && ((m >> j) & 1)) S::store(dx + j * st.cs, LpVec<T>::pack(dt));
+      if constexpr (FULL) {
+        float y[VEC], f[VEC], sc[VEC], sg[VEC];
+        st.get(s, 3, j, y);
+        if (p.scale_v) {
+          st.param(p.scale_v, j, sc);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) sc[i] = p.scale;
+        }
+        if (p.post) {
+          st.param(p.post, j, f);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) f[i] = 1.f;
+        }
+        if (p.gate) {
+          st.get(s, 4, j, sg);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float q = sigmoid_mufu(sg[i]), d = dt[i] * q;
+            sg[i] = d * sc[i] * (y[i] * rsy * f[i]) * (1.f - q);
+            dt[i] = d;
+          }
+          if (p.dgate && ((m >> j) & 1))
+            S::store(static_cast<T*>(p.dgate) + row * D + st.c0 + j * st.cs, LpVec<T>::pack(sg));
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float yh = y[i] * rsy, d = dt[i] * sc[i], e = d * f[i];
+          acc[2][j * VEC + i] = fmaf(dt[i], yh * f[i], acc[2][j * VEC + i]);
+          acc[1][j * VEC + i] = fmaf(d, yh, acc[1][j * VEC + i]);
+          doty = fmaf(e, yh, doty);
+          dz[j * VEC + i] = e;
+        }
+      }
+    }
+    if constexpr (FULL) {
+      if (p.post) doty = row_sum(doty, red) * inv;
+      T* dy = static_cast<T*>(p.dy) + row * D + st.c0;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        float y[VEC];
+        if (p.post) {
+          st.get(s, 3, j, y);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) y[i] = rsy * fmaf(-y[i] * rsy, doty, dz[j * VEC + i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) y[i] = dz[j * VEC + i];
+        }
+        if (p.dy && ((m >> j) & 1)) S::store(dy + j * st.cs, LpVec<T>::pack(y));
+      }
+    }
+  }
+  cp_async_wait<0>();
+  rn_partial<FULL ? 3 : 1>(
+      p.part + (long long)blockIdx.x * 3 * D, reinterpret_cast<float*>(rn_smem), D,
+      [&](int k, float* row_buf) {
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          if ((st.mask >> j) & 1) {
+            float* q = row_buf + st.c0 + j * st.cs;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) q[i] = acc[k][j * VEC + i];
+          }
+      });
+}
+
+// ------------------------------------------------ rows at any alignment
+// Persistent CTAs as above, all of a row's loads ahead of its sums.
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) residual_norm_fwd_kernel(ResNormParams p) {
+  using R = RnRow<T>;
+  constexpr int E = R::E;
   pdl_wait();
   pdl_trigger();
   __shared__ float red[32];
-  float dw[kRnElems], dp[kRnElems], ds[kRnElems];
-#pragma unroll
-  for (int i = 0; i < kRnElems; ++i) dw[i] = dp[i] = ds[i] = 0.f;
-  float w[kRnElems];
-  R::load_f32(p.weight, p.D, w);
-  const float inv = 1.f / p.D;
-  for (long long r0 = (long long)blockIdx.x * blockDim.y; r0 < p.rows;
-       r0 += (long long)gridDim.x * blockDim.y) {
-    const long long row = r0 + threadIdx.y;
-    const bool in = row < p.rows;
-    const int D = in ? p.D : 0;
-    float dt[kRnElems];
-    if (p.dxn) {
-      R::load(p.dxn, row * p.D, D, dt);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kRnElems; ++i) dt[i] = 0.f;
-    }
-    if (p.dh) {
-      float t[kRnElems], g[kRnElems];
-      R::load(p.x, row * p.sx, D, t);
-      R::load(p.dh, row * p.D, D, g);
-      const float rs = in ? p.rstd_x[row] : 0.f;
-      float dot = 0.f;
-#pragma unroll
-      for (int i = 0; i < kRnElems; ++i) {
-        t[i] *= rs;
-        dw[i] = fmaf(g[i], t[i], dw[i]);
-        g[i] *= w[i];
-        dot = fmaf(g[i], t[i], dot);
-      }
-      dot = row_sum(dot, red) * inv;
-#pragma unroll
-      for (int i = 0; i < kRnElems; ++i) dt[i] = fmaf(rs, g[i] - t[i] * dot, dt[i]);
-    }
-    if (p.dx) R::store(p.dx, row * p.D, D, dt);
-    if (FULL) {
-      float y[kRnElems], s[kRnElems], f[kRnElems];
-      R::load(p.y, row * p.sy, D, y);
-      const float rs = p.post && in ? p.rstd_y[row] : 1.f;
-      if (p.scale_v) {
-        R::load_f32(p.scale_v, D, s);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kRnElems; ++i) s[i] = p.scale;
-      }
-      // y becomes y^; f: the post weight
-      if (p.post) {
-        R::load_f32(p.post, D, f);
-#pragma unroll
-        for (int i = 0; i < kRnElems; ++i) y[i] *= rs;
-      } else {
-#pragma unroll
-        for (int i = 0; i < kRnElems; ++i) f[i] = 1.f;
-      }
+  const int D = p.D;
+  const R r(D);
+  for (long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y; row - threadIdx.y < p.rows;
+       row += (long long)gridDim.x * blockDim.y) {
+    // rows past the end take part in the barriers only
+    const uint32_t m = row < p.rows ? r.mask : 0;
+    const bool first = row < p.rows && threadIdx.x == 0;
+    float t[E], z[E], g[E];
+    r.load(rn_at<T>(p.x, row * p.sx), m, t);
+    r.load(rn_at<T>(p.y, row * p.sy), m, z);
+    r.load(rn_at<T>(p.gate, row * p.sgate), m, g);
+    if (p.y) {
       if (p.gate) {
-        float g[kRnElems];
-        R::load(p.gate, row * p.sgate, D, g);
 #pragma unroll
-        for (int i = 0; i < kRnElems; ++i) {
-          const float sg = rn_sigmoid(g[i]);
-          g[i] = dt[i] * s[i] * y[i] * f[i] * (sg * (1.f - sg));
-          ds[i] = fmaf(dt[i] * sg, y[i] * f[i], ds[i]);
-          dt[i] *= s[i] * sg;  // dz from here on
-        }
-        if (p.dgate) R::store(p.dgate, row * p.D, D, g);
+        for (int i = 0; i < E; ++i) g[i] = sigmoid_mufu(g[i]);
       } else {
 #pragma unroll
-        for (int i = 0; i < kRnElems; ++i) {
-          ds[i] = fmaf(dt[i], y[i] * f[i], ds[i]);
-          dt[i] *= s[i];
-        }
+        for (int i = 0; i < E; ++i) g[i] = 1.f;
+      }
+      float w[E];
+      if (p.post) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) ss = fmaf(z[i], z[i], ss);
+        const float rs = rsqrtf(row_sum(ss, red) / D + p.eps);
+        r.param(p.post, w);
+#pragma unroll
+        for (int i = 0; i < E; ++i) z[i] = z[i] * rs * w[i];
+        if (first && p.rstd_y) p.rstd_y[row] = rs;
+      }
+      if (p.scale_v) {
+        r.param(p.scale_v, w);
+#pragma unroll
+        for (int i = 0; i < E; ++i) g[i] *= w[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) g[i] *= p.scale;
+      }
+      // the norm reads the stream as it is kept, in x's type
+#pragma unroll
+      for (int i = 0; i < E; ++i) t[i] = rn_round<T>(fmaf(g[i], z[i], t[i]));
+      r.store(static_cast<T*>(p.xn) + row * D, m, t);
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) ss = fmaf(t[i], t[i], ss);
+    const float rs = rsqrtf(row_sum(ss, red) / D + p.eps);
+    if (first && p.rstd_x) p.rstd_x[row] = rs;
+    r.param(p.weight, g);
+#pragma unroll
+    for (int i = 0; i < E; ++i) t[i] = t[i] * rs * g[i];
+    r.store(static_cast<T*>(p.h) + row * D, m, t);
+  }
+}
+
+// p.x is the new stream x'.
+template <typename T, int THREADS, bool FULL>
+__global__ void __launch_bounds__(THREADS) residual_norm_bwd_kernel(ResNormParams p) {
+  using R = RnRow<T>;
+  constexpr int E = R::E;
+  extern __shared__ __align__(16) uint8_t rn_smem[];
+  __shared__ float red[32];
+  pdl_wait();
+  pdl_trigger();
+  const int D = p.D;
+  const R r(D);
+  float acc[FULL ? 3 : 1][E];  // dweight, dpost, dscale
+#pragma unroll
+  for (int k = 0; k < (FULL ? 3 : 1); ++k)
+#pragma unroll
+    for (int i = 0; i < E; ++i) acc[k][i] = 0.f;
+  const float inv = 1.f / D;
+  for (long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y; row - threadIdx.y < p.rows;
+       row += (long long)gridDim.x * blockDim.y) {
+    const bool in = row < p.rows;
+    const uint32_t m = in ? r.mask : 0;
+    float t[E], g[E], dt[E], y[E], sg[E], w[E];
+    r.load(rn_at<T>(p.x, row * p.sx), m, t);
+    r.load(rn_at<T>(p.dh, row * D), m, g);
+    r.load(rn_at<T>(p.dxn, row * D), m, dt);
+    if (FULL) {
+      r.load(rn_at<T>(p.y, row * p.sy), m, y);
+      r.load(rn_at<T>(p.gate, row * p.sgate), m, sg);
+    }
+    const float rs = in ? p.rstd_x[row] : 0.f;
+    const float rsy = FULL && p.post && in ? p.rstd_y[row] : 1.f;
+    r.param(p.weight, w);
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      t[i] *= rs;
+      acc[0][i] = fmaf(g[i], t[i], acc[0][i]);
+      g[i] *= w[i];
+      dot = fmaf(g[i], t[i], dot);
+    }
+    dot = row_sum(dot, red) * inv;
+#pragma unroll
+    for (int i = 0; i < E; ++i) dt[i] = fmaf(rs, fmaf(-t[i], dot, g[i]), dt[i]);
+    if (p.dx) r.store(static_cast<T*>(p.dx) + row * D, m, dt);
+    if constexpr (FULL) {
+      // t: scale, w: post weight, g: gate
+      if (p.scale_v) {
+        r.param(p.scale_v, t);
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) t[i] = p.scale;
       }
       if (p.post) {
-        float dot = 0.f;
+        r.param(p.post, w);
+      } else {
 #pragma unroll
-        for (int i = 0; i < kRnElems; ++i) {
-          dp[i] = fmaf(dt[i], y[i], dp[i]);
-          dt[i] *= f[i];
-          dot = fmaf(dt[i], y[i], dot);
+        for (int i = 0; i < E; ++i) w[i] = 1.f;
+      }
+#pragma unroll
+      for (int i = 0; i < E; ++i) y[i] *= rsy;
+      if (p.gate) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const float q = sigmoid_mufu(sg[i]);
+          dt[i] *= q;
+          sg[i] = dt[i] * t[i] * (y[i] * w[i]) * (1.f - q);
         }
-        dot = row_sum(dot, red) * inv;
-#pragma unroll
-        for (int i = 0; i < kRnElems; ++i) dt[i] = rs * (dt[i] - y[i] * dot);
+        if (p.dgate) r.store(static_cast<T*>(p.dgate) + row * D, m, sg);
       }
-      if (p.dy) R::store(p.dy, row * p.D, D, dt);
+      float doty = 0.f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        acc[2][i] = fmaf(dt[i], y[i] * w[i], acc[2][i]);
+        dt[i] *= t[i];
+        acc[1][i] = fmaf(dt[i], y[i], acc[1][i]);
+        dt[i] *= w[i];
+        doty = fmaf(dt[i], y[i], doty);
+      }
+      if (p.post) {
+        doty = row_sum(doty, red) * inv;
+#pragma unroll
+        for (int i = 0; i < E; ++i) dt[i] = rsy * fmaf(-y[i], doty, dt[i]);
+      }
+      if (p.dy) r.store(static_cast<T*>(p.dy) + row * D, m, dt);
     }
   }
-  // one partial row per (CTA, row slot)
-  float* out = p.part + ((long long)blockIdx.x * blockDim.y + threadIdx.y) * 3 * p.D;
+  rn_partial<FULL ? 3 : 1>(p.part + (long long)blockIdx.x * 3 * D, reinterpret_cast<float*>(rn_smem), D,
+                           [&](int k, float* row_buf) {
 #pragma unroll
-  for (int j = 0; j < R::J; ++j) {
-    const int c = R::col(j);
-    if (c >= p.D) continue;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      out[c + i] = dw[j * VEC + i];
-      if (FULL) {
-        out[p.D + c + i] = dp[j * VEC + i];
-        out[2 * p.D + c + i] = ds[j * VEC + i];
-      }
-    }
-  }
+                             for (int j = 0; j < E; ++j)
+                               if ((r.mask >> j) & 1) row_buf[r.off[j]] = acc[k][j];
+                           });
 }
 
 // Column sums of the partial rows, in a fixed order: CTA (32 columns, set),
@@ -292,39 +574,65 @@ __global__ void __launch_bounds__(1024)
   if (threadIdx.x == 0 && cc < D) out[cc] = v;
 }
 
-constexpr int kRnMaxParts = 148 * 8;  // partial rows of the backward
-
-// threads of a row and rows of a CTA
-static dim3 rn_block(int D, long long rows) {
-  const int tx = ((D + kRnElems - 1) / kRnElems + 31) / 32 * 32;
+// threads of a row with E columns each, and rows of a CTA
+static dim3 rn_block(int D, int E, long long rows) {
+  const int tx = ((D + E - 1) / E + 31) / 32 * 32;
   int ty = 1;
   while (ty < 8 && tx * ty * 2 <= 256 && rows > ty) ty *= 2;
   return dim3(unsigned(tx), unsigned(ty));
 }
-
-static int rn_vec(int D, int es, std::initializer_list<const void*> ptrs,
-                  std::initializer_list<long long> strides) {
-  int vec = 16 / es;
-  for (; vec > 1; vec /= 2) {
-    bool ok = D % vec == 0;
-    for (const void* q : ptrs) ok = ok && (!q || aligned(q, size_t(vec) * es));
-    for (long long st : strides) ok = ok && st % vec == 0;
-    if (ok) break;
+// Columns of a thread: 8, or 32 with 16-byte accesses once 8 would be more than a warp
+// a row (8192 columns are 256 threads); with y's side 16-byte accesses keep 16, for
+// the three accumulators a column.
+static int rn_elems(int D, int vec, bool full) {
+  return vec == 1 || D <= 256 ? 8 : (full && D <= 4096 ? 16 : 32);
+}
+// shared memory of one slot of a row's tensors; two slots where they fit (they do not
+// for four or five fp32 tensors of more than 5600 columns)
+static size_t rn_slot_bytes(dim3 block, int elems, int es, int tensors) {
+  return size_t(tensors) * elems * es * block.x * block.y;
+}
+constexpr int kRnMaxSmem = 226 << 10;
+static int rn_stages(size_t slot) { return 2 * slot <= kRnMaxSmem ? 2 : 1; }
+// CTAs an SM holds at a time (shared memory and registers)
+static int rn_per_sm(dim3 block, int vec, size_t smem) {
+  const int threads = int(block.x * block.y);
+  if (vec == 1) return std::max(1, 1024 / threads);
+  return int(std::max<size_t>(1, std::min<size_t>(std::min<size_t>(4, 768 / threads),
+                                                  (220 << 10) / (smem + 1024))));
+}
+struct RnBwdShape {
+  int elems, stages;
+  dim3 block;
+  size_t smem;
+  unsigned grid;
+  RnBwdShape(int D, int es, long long rows, bool full, bool gate, int vec) {
+    elems = rn_elems(D, vec, full);
+    block = rn_block(D, elems, rows);
+    const size_t slot = rn_slot_bytes(block, elems, es, full ? 4 + gate : 3);
+    stages = rn_stages(slot);
+    smem = vec == 1 ? block.y * D * sizeof(float) : stages * slot;
+    grid = unsigned(std::min<long long>((rows + block.y - 1) / block.y,
+                                        148ll * rn_per_sm(block, vec, smem)));
   }
-  // the kernels are built for the full width and for single elements
-  return vec == 16 / es ? vec : 1;
+};
+
+// 16-byte accesses where every row and parameter allows them, else single elements
+static int rn_vec(int D, int es, std::initializer_list<const void*> ptrs,
+                  std::initializer_list<const float*> params,
+                  std::initializer_list<long long> strides) {
+  const int vec = 16 / es;
+  bool ok = D % vec == 0;
+  for (const void* q : ptrs) ok = ok && aligned(q, 16);
+  for (const float* q : params) ok = ok && aligned(q, 16);
+  for (long long st : strides) ok = ok && st % vec == 0;
+  return ok ? vec : 1;
 }
 
 static int rn_checks(int dtype, long long rows, int D) {
   CYFA_REQUIRE(rows > 0 && rows < (1ll << 31) && D > 0 && D <= kRnMaxWidth, kBadShape);
   CYFA_REQUIRE(dtype == 0 || dtype == 1, kBadDtype);
   return kOk;
-}
-
-static unsigned rn_bwd_grid(dim3 block, long long rows) {
-  const int per_sm = std::max(1, 1024 / int(block.x * block.y));
-  const long long ctas = (rows + block.y - 1) / block.y;
-  return unsigned(std::min<long long>({ctas, 148ll * per_sm, (long long)kRnMaxParts / block.y}));
 }
 
 }  // namespace cyfa
@@ -359,18 +667,42 @@ int cyfa_residual_norm_fwd(const cyfa_residual_norm_args* a, void* xn, void* h, 
   p.h = h;
   p.rstd_x = rstd_x;
   p.rstd_y = rstd_y;
-  const dim3 block = rn_block(a->D, a->rows);
-  const unsigned grid = unsigned((a->rows + block.y - 1) / block.y);
-  const int vec = rn_vec(a->D, es, {a->x, a->y, a->gate, xn, h},
+  const int vec = rn_vec(a->D, es, {a->x, a->y, a->gate, xn, h}, {a->weight, a->post_weight, a->scale_vector},
                          {a->x_stride, a->y ? a->y_stride : 0, a->gate ? a->gate_stride : 0});
+  const int elems = rn_elems(a->D, vec, false);
+  const dim3 block = rn_block(a->D, elems, a->rows);
+  const long long ctas = (a->rows + block.y - 1) / block.y;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-#define CYFA_RN(T, VEC)            \
+  if (vec > 1) {
+    const size_t slot = rn_slot_bytes(block, elems, es, 1 + (a->y != nullptr) + (a->gate != nullptr));
+    p.stages = rn_stages(slot);
+    const size_t smem = p.stages * slot;
+    const unsigned grid = unsigned(std::min<long long>(ctas, 148ll * rn_per_sm(block, vec, smem)));
+    const bool plain = a->y && !a->post_weight && !a->gate && !a->scale_vector && a->scale == 1.f;
+#define CYFA_RN_L(T, E, PLAIN)                                                                       \
+  do {                                                                                               \
+    set_smem(residual_norm_fwd_stream_kernel<T, E, PLAIN>, kRnMaxSmem);                              \
+    CYFA_LAUNCH("residual_norm_fwd", s,                                                              \
+                (launch_k(residual_norm_fwd_stream_kernel<T, E, PLAIN>, grid, block, smem, s, p)));  \
+  } while (0)
+#define CYFA_RN(T, E) \
+  do { if (plain) CYFA_RN_L(T, E, true); else CYFA_RN_L(T, E, false); } while (0)
+    if (a->dtype == 1) {
+      if (elems == 8) CYFA_RN(__nv_bfloat16, 8); else CYFA_RN(__nv_bfloat16, 32);
+    } else {
+      if (elems == 8) CYFA_RN(float, 8); else CYFA_RN(float, 32);
+    }
+#undef CYFA_RN
+#undef CYFA_RN_L
+    return launch_status();
+  }
+#define CYFA_RN(T, THREADS)            \
   CYFA_LAUNCH("residual_norm_fwd", s, \
-              (launch_k(residual_norm_fwd_kernel<T, VEC>, grid, block, 0, s, p)))
+              (launch_k(residual_norm_fwd_kernel<T, THREADS>, unsigned(std::min<long long>(ctas, 148 * rn_per_sm(block, 1, 0))), block, 0, s, p)))
   if (a->dtype == 1) {
-    if (vec == 8) CYFA_RN(__nv_bfloat16, 8); else CYFA_RN(__nv_bfloat16, 1);
+    if (block.x > 256) CYFA_RN(__nv_bfloat16, 1024); else CYFA_RN(__nv_bfloat16, 256);
   } else {
-    if (vec == 4) CYFA_RN(float, 4); else CYFA_RN(float, 1);
+    if (block.x > 256) CYFA_RN(float, 1024); else CYFA_RN(float, 256);
   }
 #undef CYFA_RN
   return launch_status();
@@ -378,8 +710,12 @@ int cyfa_residual_norm_fwd(const cyfa_residual_norm_args* a, void* xn, void* h, 
 
 size_t cyfa_residual_norm_bwd_work_bytes(long long rows, int D) {
   if (rows <= 0 || D <= 0 || D > kRnMaxWidth) return 0;
-  const dim3 block = rn_block(D, rows);
-  return size_t(rn_bwd_grid(block, rows)) * block.y * 3 * D * sizeof(float);
+  size_t most = 0;
+  for (int k = 0; k < 16; ++k) {
+    const RnBwdShape sh(D, k & 1 ? 2 : 4, rows, k & 2, k & 4, k & 8 ? 4 : 1);
+    most = std::max(most, size_t(sh.grid));
+  }
+  return most * 3 * D * sizeof(float);
 }
 
 int cyfa_residual_norm_bwd(const cyfa_residual_norm_args* a, const float* rstd_x,
@@ -419,32 +755,45 @@ int cyfa_residual_norm_bwd(const cyfa_residual_norm_args* a, const float* rstd_x
   p.dy = dy;
   p.dgate = dgate;
   p.part = static_cast<float*>(work);
-  const dim3 block = rn_block(a->D, a->rows);
-  const unsigned grid = rn_bwd_grid(block, a->rows);
-  const int vec = rn_vec(a->D, es, {a->x, a->y, a->gate, dxn, dh, dx, dy, dgate},
-                         {a->x_stride, a->y ? a->y_stride : 0, a->gate ? a->gate_stride : 0});
   // without gate, scale and post-norm, dy equals dx: the plain sum's gradient
   const bool full = a->y && (dy || dgate || dpost || dscale);
+  const int vec = rn_vec(a->D, es, {a->x, a->y, a->gate, dxn, dh, dx, dy, dgate},
+                         {a->weight, a->post_weight, a->scale_vector},
+                         {a->x_stride, a->y ? a->y_stride : 0, a->gate ? a->gate_stride : 0});
+  const RnBwdShape sh(a->D, es, a->rows, full, a->gate != nullptr, vec);
+  p.stages = sh.stages;
+  const dim3 block = sh.block;
+  const unsigned grid = sh.grid;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-#define CYFA_RN(T, VEC)                                                                        \
-  do {                                                                                         \
-    if (full)                                                                                  \
-      CYFA_LAUNCH("residual_norm_bwd", s,                                                      \
-                  (launch_k(residual_norm_bwd_kernel<T, VEC, true>, grid, block, 0, s, p)));   \
-    else                                                                                       \
-      CYFA_LAUNCH("residual_norm_bwd", s,                                                      \
-                  (launch_k(residual_norm_bwd_kernel<T, VEC, false>, grid, block, 0, s, p)));  \
+#define CYFA_RN_S(T, E, FULL)                                                                        \
+  do {                                                                                               \
+    set_smem(residual_norm_bwd_stream_kernel<T, E, FULL>, kRnMaxSmem);                               \
+    CYFA_LAUNCH("residual_norm_bwd", s,                                                              \
+                (launch_k(residual_norm_bwd_stream_kernel<T, E, FULL>, grid, block, sh.smem, s, p))); \
+  } while (0)
+#define CYFA_RN_L(T, THREADS, FULL)    \
+  CYFA_LAUNCH("residual_norm_bwd", s, \
+              (launch_k(residual_norm_bwd_kernel<T, THREADS, FULL>, grid, block, sh.smem, s, p)))
+#define CYFA_RN(T, FULL)                                        \
+  do {                                                          \
+    if (vec > 1 && sh.elems == 8) CYFA_RN_S(T, 8, FULL);        \
+    else if (vec > 1 && sh.elems == 16) CYFA_RN_S(T, 16, FULL); \
+    else if (vec > 1) CYFA_RN_S(T, 32, FULL);                   \
+    else if (block.x > 256) CYFA_RN_L(T, 1024, FULL);           \
+    else CYFA_RN_L(T, 256, FULL);                               \
   } while (0)
   if (a->dtype == 1) {
-    if (vec == 8) CYFA_RN(__nv_bfloat16, 8); else CYFA_RN(__nv_bfloat16, 1);
+    if (full) CYFA_RN(__nv_bfloat16, true); else CYFA_RN(__nv_bfloat16, false);
   } else {
-    if (vec == 4) CYFA_RN(float, 4); else CYFA_RN(float, 1);
+    if (full) CYFA_RN(float, true); else CYFA_RN(float, false);
   }
 #undef CYFA_RN
+#undef CYFA_RN_L
+#undef CYFA_RN_S
   if (dweight || dpost || dscale)
     CYFA_LAUNCH("residual_norm_sum", s,
                 (launch_k(residual_norm_sum_kernel, dim3(unsigned((a->D + 31) / 32), 3), dim3(32, 32),
-                          0, s, p.part, int(grid * block.y), a->D, dweight, dpost, dscale)));
+                          0, s, p.part, int(grid), a->D, dweight, dpost, dscale)));
   return launch_status();
 }
 
