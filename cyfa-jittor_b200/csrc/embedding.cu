@@ -37,30 +37,45 @@ struct EmbVec {
   }
 };
 
+// CTA: kEmbItems accesses of VEC elements in a row-major walk over the output; a
+// thread's accesses are all in flight together.
+template <int VEC>
+constexpr int emb_unroll() {
+  return VEC >= 4 ? 4 : 8;
+}
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kEmbThreads)
     embed_fwd_kernel(const long long* tokens, const T* w, T* out, long long N, long long V, int D,
                      float scale) {
+  constexpr int U = emb_unroll<VEC>();
   pdl_wait();
   pdl_trigger();
-  const int per_row = D / VEC;
-  const long long total = N * per_row;
-  for (long long i = (long long)blockIdx.x * kEmbThreads + threadIdx.x; i < total;
-       i += (long long)gridDim.x * kEmbThreads) {
-    const long long n = i / per_row;
-    const int c = int(i - n * per_row) * VEC;
-    const long long id = tokens[n];
-    float f[VEC];
-    if (id >= 0 && id < V) {
-      EmbVec<T, VEC>::load(w + id * D + c, f);
+  const unsigned per_row = unsigned(D / VEC);
+  const long long first = (long long)blockIdx.x * (U * kEmbThreads), n0 = first / per_row;
+  const unsigned rem = unsigned(first - n0 * per_row);
+  float f[U][VEC];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) f[k] *= scale;
-    } else {
+  for (int k = 0; k < U; ++k) {
+    const unsigned i = rem + k * kEmbThreads + threadIdx.x, r = i / per_row;
+    const long long n = n0 + r;
+    const unsigned c = (i - r * per_row) * VEC;
+    if (n < N) {
+      const long long id = __ldg(tokens + n);
+      if (id >= 0 && id < V) {
+        EmbVec<T, VEC>::load(w + id * D + c, f[k]);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) f[k] = 0.f;
-      if (c == 0) set_error(kErrBadIndex);
+        for (int e = 0; e < VEC; ++e) f[k][e] *= scale;
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[k][e] = 0.f;
+        if (c == 0) set_error(kErrBadIndex);
+      }
     }
-    EmbVec<T, VEC>::store(out + n * D + c, f);
+  }
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const long long i = first + k * kEmbThreads + threadIdx.x;
+    if (i < N * per_row) EmbVec<T, VEC>::store(out + i * VEC, f[k]);
   }
 }
 
@@ -181,6 +196,164 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_move_kernel(SortPass 
   }
 }
 
+// The whole sort in one cluster of 8 CTAs, for up to kCsMax tokens: the entries live
+// in the CTAs' shared memory, a thread holds its own in registers while a pass
+// scatters them to their places, in whichever CTA.  A pass takes three cluster
+// barriers instead of three launches.  The grid's other clusters clear the
+// table's gradient meanwhile.
+constexpr int kCsCtas = 8;
+constexpr int kCsThreads = 1024;
+constexpr int kCsWarps = kCsThreads / 32;
+constexpr int kCsDigits = 512;
+constexpr int kCsClear = 2048;   // vectors of one clearing copy
+constexpr int kCsMaxPer = 16;  // entries of a thread
+constexpr long long kCsMax = (long long)kCsCtas * kCsThreads * kCsMaxPer;
+
+struct ClusterSortParams {
+  const long long* tokens;
+  uint32_t *key_out, *pos_out;
+  long long N, V, pad;
+  int bits, passes;       // digit width, passes
+  uint4* clear;           // table gradient from its first 16-byte boundary
+  long long clear_vecs;
+  uint8_t *edge0, *edge1;  // bytes before and after
+  int edge0_bytes, edge1_bytes;
+};
+
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
+               "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+}
+template <int PER>
+constexpr int cs_smem() {
+  return kCsThreads * PER * 8 + kCsWarps * kCsDigits * 2 + kCsDigits * 8 + 64 * 4;
+}
+
+template <int PER>
+__global__ void __launch_bounds__(kCsThreads) embed_cluster_sort_kernel(ClusterSortParams p) {
+  constexpr int kChunk = kCsThreads * PER;
+  extern __shared__ __align__(16) uint8_t cs_smem_raw[];
+  uint2* entry = reinterpret_cast<uint2*>(cs_smem_raw);                       // [kChunk] key, position
+  uint16_t* run = reinterpret_cast<uint16_t*>(entry + kChunk);                // [warps][digits]
+  uint32_t* count = reinterpret_cast<uint32_t*>(run + kCsWarps * kCsDigits);  // [digits] of this CTA
+  uint32_t* base = count + kCsDigits;                                         // [digits]
+  uint32_t* part = base + kCsDigits;
+  pdl_wait();
+  pdl_trigger();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (blockIdx.x >= kCsCtas) {
+    const long long i0 = (long long)(blockIdx.x - kCsCtas) * kCsThreads + tid;
+    const long long step = (long long)(gridDim.x - kCsCtas) * kCsThreads;
+    // 32 KiB of zeros in shared memory, stored over and over by bulk copies
+    uint4* zeros = reinterpret_cast<uint4*>(cs_smem_raw);
+    for (int i = tid; i < kCsClear; i += kCsThreads) zeros[i] = make_uint4(0, 0, 0, 0);
+    fence_async_smem();
+    __syncthreads();
+    if (tid == 0) {
+      for (long long v = (i0 / kCsThreads) * kCsClear; v < p.clear_vecs;
+           v += (step / kCsThreads) * kCsClear)
+        bulk_store(p.clear + v, zeros, uint32_t(min((long long)kCsClear, p.clear_vecs - v)) * 16);
+      bulk_commit();
+      bulk_wait_all();
+    }
+    if (i0 < p.edge0_bytes) p.edge0[i0] = 0;
+    if (i0 < p.edge1_bytes) p.edge1[i0] = 0;
+    return;
+  }
+  const uint32_t rank = cluster_rank();
+  const uint32_t mask = (1u << p.bits) - 1, ndig = 1u << p.bits;
+  // warp w of CTA r holds the entries (r 32 + w) 32 PER .., in rounds of 32
+  const long long n0 = (long long)rank * kChunk + warp * (32 * PER) + lane;
+  uint2 e[PER];
+#pragma unroll
+  for (int r = 0; r < PER; ++r) {
+    const long long n = n0 + r * 32;
+    // past the end: after every key
+    e[r] = n < p.N ? make_uint2(sort_key(p.tokens, p.V, p.pad, n), uint32_t(n))
+                   : make_uint2(0xffffffffu, 0xffffffffu);
+  }
+  for (int pass = 0; pass < p.passes; ++pass) {
+    const int shift = pass * p.bits;
+    for (uint32_t d = lane; d < ndig; d += 32) run[warp * kCsDigits + d] = 0;
+    __syncwarp();
+    uint16_t before[PER];  // entries of the digit earlier in the warp's run
+#pragma unroll
+    for (int r = 0; r < PER; ++r) {
+      const uint32_t d = (e[r].x >> shift) & mask;
+      const unsigned same = __match_any_sync(0xffffffffu, d);
+      const uint16_t c = run[warp * kCsDigits + d];
+      before[r] = uint16_t(c + __popc(same & ((1u << lane) - 1)));
+      __syncwarp();
+      if (lane == __ffs(same) - 1) run[warp * kCsDigits + d] = uint16_t(c + __popc(same));
+      __syncwarp();
+    }
+    __syncthreads();
+    // runs' offsets inside the CTA, and the CTA's count, per digit
+    if (tid < int(ndig)) {
+      uint32_t sum = 0;
+#pragma unroll 8
+      for (int w = 0; w < kCsWarps; ++w) {
+        const uint32_t c = run[w * kCsDigits + tid];
+        run[w * kCsDigits + tid] = uint16_t(sum);
+        sum += c;
+      }
+      count[tid] = sum;
+    }
+    cluster_sync_all();  // the counts are there, and every entry is in registers
+    {
+      uint32_t total = 0, mine = 0;
+      if (tid < int(ndig)) {
+#pragma unroll
+        for (uint32_t c = 0; c < kCsCtas; ++c) {
+          const uint32_t v = cluster_ld_u32(cluster_map(smem_u32(count + tid), c));
+          if (c < rank) mine += v;
+          total += v;
+        }
+      }
+      uint32_t inc = total;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      if (lane == 31) part[warp] = inc;
+      __syncthreads();
+      if (warp == 0) {
+        const uint32_t v = part[lane];
+        uint32_t s = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t t = __shfl_up_sync(0xffffffffu, s, o);
+          if (lane >= o) s += t;
+        }
+        part[lane] = s - v;
+      }
+      __syncthreads();
+      if (tid < int(ndig)) base[tid] = part[warp] + inc - total + mine;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < PER; ++r) {
+      const uint32_t d = (e[r].x >> shift) & mask;
+      const uint32_t at = base[d] + run[warp * kCsDigits + d] + before[r];
+      cluster_st_u2(cluster_map(smem_u32(entry + at % kChunk), at / kChunk), e[r]);
+    }
+    cluster_sync_all();  // every entry is in its place
+#pragma unroll
+    for (int r = 0; r < PER; ++r) e[r] = entry[warp * (32 * PER) + r * 32 + lane];
+  }
+#pragma unroll
+  for (int r = 0; r < PER; ++r) {
+    const long long n = n0 + r * 32;
+    if (n < p.N) {
+      p.key_out[n] = e[r].x;
+      p.pos_out[n] = e[r].y;
+    }
+  }
+  cluster_sync_all();  // no CTA leaves while its shared memory may be written
+}
+
 // ------------------------------------------------------------------- the sums
 // The sorted entries in pieces of kPiece: CTA (piece, columns) adds the rows of
 // each run of equal ids.  A run inside the piece is written at once.  A run that
@@ -205,6 +378,7 @@ struct EmbSumParams {
 
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kSumThreads) embed_sum_kernel(EmbSumParams p) {
+  constexpr int kBatch = 8;
   pdl_wait();
   pdl_trigger();
   __shared__ uint32_t key[kPiece + 2], pos[kPiece];  // key[0]: the entry before, key[cnt + 1]: after
@@ -223,54 +397,96 @@ __global__ void __launch_bounds__(kSumThreads) embed_sum_kernel(EmbSumParams p) 
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
   bool opened = key[0] == key[1];  // the current run began in an earlier piece
-#pragma unroll 4
-  for (int i = 0; i < cnt; ++i) {
-    const uint32_t v = key[i + 1];
-    if (v >= p.V) break;  // the dropped entries: nothing after them counts
-    float f[VEC];
-    EmbVec<T, VEC>::load(src + (size_t)pos[i] * p.D, f);
+  // rows in batches, a batch's loads ahead of its sums
+  for (int i0 = 0; i0 < cnt && key[i0 + 1] < p.V; i0 += kBatch) {
+    float f[kBatch][VEC];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) acc[k] += f[k];
-    if (key[i + 2] == v && i + 1 < cnt) continue;
-    const bool goes_on = key[i + 2] == v;
-    if (opened || goes_on) {
-      float* d = (opened ? p.head : p.tail) + (size_t)blockIdx.x * p.D + c;
+    for (int b = 0; b < kBatch; ++b)
+      if (i0 + b < cnt && key[i0 + b + 1] < p.V)
+        EmbVec<T, VEC>::load(src + (size_t)pos[i0 + b] * p.D, f[b]);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) d[k] = acc[k];
-    } else {
+    for (int b = 0; b < kBatch; ++b) {
+      const int i = i0 + b;
+      if (i >= cnt) break;
+      const uint32_t v = key[i + 1];
+      if (v >= p.V) break;  // the dropped entries: nothing after them counts
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) acc[k] *= p.scale;
-      EmbVec<T, VEC>::store(static_cast<T*>(p.dw) + (size_t)v * p.D + c, acc);
+      for (int k = 0; k < VEC; ++k) acc[k] += f[b][k];
+      const bool goes_on = key[i + 2] == v;
+      if (goes_on && i + 1 < cnt) continue;
+      if (opened || goes_on) {
+        float* d = (opened ? p.head : p.tail) + (size_t)blockIdx.x * p.D + c;
+        if (VEC % 4 == 0) {  // D is a multiple of VEC
+#pragma unroll
+          for (int k = 0; k + 3 < VEC; k += 4)
+            *reinterpret_cast<float4*>(d + k) = make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) d[k] = acc[k];
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] *= p.scale;
+        EmbVec<T, VEC>::store(static_cast<T*>(p.dw) + (size_t)v * p.D + c, acc);
+      }
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+      opened = false;
     }
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-    opened = false;
   }
 }
 
-// CTA (piece, columns): if a run begins in the piece and goes on, the run's
-// parts in order: tail[piece], then head of the pieces up to its end.
-template <typename T>
+// CTA (piece, 32 VEC columns at a time): if a run begins in the piece and goes on,
+// the run's parts: tail[piece], then head of the pieces up to its end, in 8
+// stretches side by side that are added in order.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(256) embed_join_kernel(EmbSumParams p) {
+  __shared__ float sum[8][32 * VEC];
   pdl_wait();
   pdl_trigger();
   const long long b = blockIdx.x;
   const long long last = b * kPiece + kPiece - 1;  // the piece's last entry
   if (last + 1 >= p.N) return;
-  const uint32_t v = p.key[last];
-  if (v >= p.V || p.key[last + 1] != v) return;
-  if (b > 0 && p.key[b * kPiece] == v && p.key[b * kPiece - 1] == v) return;  // began earlier
+  const uint32_t v = p.key[last], next = p.key[last + 1], first = p.key[b * kPiece];
+  const uint32_t prev = b > 0 ? p.key[b * kPiece - 1] : 0xffffffffu;
+  if (v >= p.V || next != v) return;
+  if (first == v && prev == v) return;  // began earlier
   long long lo = last + 1, hi = p.N - 1;  // last entry of the run
   while (lo < hi) {
     const long long mid = (lo + hi + 1) >> 1;
     if (p.key[mid] <= v) lo = mid; else hi = mid - 1;
   }
-  const long long end = lo / kPiece;
-  const int c = blockIdx.y * 256 + threadIdx.x;
-  if (c >= p.D) return;
-  float acc = p.tail[(size_t)b * p.D + c];
-  for (long long q = b + 1; q <= end; ++q) acc += p.head[(size_t)q * p.D + c];
-  static_cast<T*>(p.dw)[(size_t)v * p.D + c] = T(acc * p.scale);
+  const long long parts = lo / kPiece - b, per = (parts + 7) / 8;  // head pieces
+  const int col = (threadIdx.x & 31) * VEC, g = threadIdx.x >> 5;
+  for (int c0 = blockIdx.y * 32 * VEC; c0 < p.D; c0 += gridDim.y * 32 * VEC) {
+    const int c = c0 + col;
+    float acc[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+    if (c < p.D) {
+      if (g == 0) EmbVec<float, VEC>::load(p.tail + (size_t)b * p.D + c, acc);
+      const long long e = min(parts, (g + 1) * per);
+#pragma unroll 4
+      for (long long q = g * per; q < e; ++q) {
+        float f[VEC];
+        EmbVec<float, VEC>::load(p.head + (size_t)(b + 1 + q) * p.D + c, f);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] += f[k];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) sum[g][col + k] = acc[k];
+    __syncthreads();
+    if (g == 0 && c < p.D) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+#pragma unroll
+        for (int j = 1; j < 8; ++j) acc[k] += sum[j][col + k];
+        static_cast<T*>(p.dw)[(size_t)v * p.D + c + k] = T(acc[k] * p.scale);
+      }
+    }
+    __syncthreads();
+  }
 }
 
 static size_t embed_align(size_t n) { return (n + 255) / 256 * 256; }
@@ -324,8 +540,9 @@ int cyfa_embed_fwd(const long long* tokens, const void* weight, int dtype, void*
   const int es = dtype == 1 ? 2 : 4;
   CYFA_REQUIRE(aligned(tokens, 8) && aligned(weight, es) && aligned(out, es), kMisaligned);
   const int vec = embed_vec(D, es, weight, out);
-  const long long n = N * (D / vec);
-  const unsigned grid = unsigned(std::min<long long>((n + kEmbThreads - 1) / kEmbThreads, 148 * 64));
+  const long long n = N * (D / vec), per_cta = (vec >= 4 ? 4 : 8) * kEmbThreads;
+  CYFA_REQUIRE((n + per_cta - 1) / per_cta < (1ll << 31), kBadShape);
+  const unsigned grid = unsigned((n + per_cta - 1) / per_cta);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
 #define CYFA_EMB(T, VEC)                                                                       \
   CYFA_LAUNCH("embed_fwd", s,                                                                  \
@@ -361,25 +578,64 @@ int cyfa_embed_bwd(const long long* tokens, const void* dout, int dtype, void* d
   const EmbWork w(work, N, D);
   CYFA_REQUIRE(work_bytes >= w.bytes, kWorkspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = cudaMemsetAsync(dweight, 0, size_t(V) * D * es, s);
-  if (e != cudaSuccess) return -static_cast<int>(e);
-  SortPass p{tokens, nullptr, nullptr, w.key[0], w.pos[0], w.count, N, V, padding_idx, 0,
-             int((N + kSortTile - 1) / kSortTile)};
   int cur = 0;
-  for (int shift = 0; shift < 32 && (V >> shift) > 0; shift += 8) {
-    p.shift = shift;
-    CYFA_LAUNCH("embed_sort_count", s,
-                (launch_k(embed_sort_count_kernel, unsigned(p.tiles), kSortThreads, 0, s, p)));
-    CYFA_LAUNCH("embed_sort_scan", s,
-                (launch_k(embed_sort_scan_kernel, 1, 1024, 0, s, w.count, p.tiles * 256)));
-    CYFA_LAUNCH("embed_sort_move", s,
-                (launch_k(embed_sort_move_kernel, unsigned(p.tiles), kSortThreads, 0, s, p)));
-    cur = p.key_out == w.key[0] ? 0 : 1;
-    p.tokens = nullptr;
-    p.key_in = w.key[cur];
-    p.pos_in = w.pos[cur];
-    p.key_out = w.key[1 - cur];
-    p.pos_out = w.pos[1 - cur];
+  if (N <= kCsMax) {
+    ClusterSortParams p{};
+    p.tokens = tokens;
+    p.key_out = w.key[0];
+    p.pos_out = w.pos[0];
+    p.N = N;
+    p.V = V;
+    p.pad = padding_idx;
+    int bits = 1;  // of the largest key, V
+    while ((V >> bits) > 0) ++bits;
+    p.passes = (bits + 8) / 9;
+    p.bits = (bits + p.passes - 1) / p.passes;
+    uint8_t* d = static_cast<uint8_t*>(dweight);
+    const size_t nbytes = size_t(V) * D * es;
+    const size_t lead = std::min(nbytes, (16 - reinterpret_cast<uintptr_t>(d) % 16) % 16);
+    p.edge0 = d;
+    p.edge0_bytes = int(lead);
+    p.clear = reinterpret_cast<uint4*>(d + lead);
+    p.clear_vecs = (long long)((nbytes - lead) / 16);
+    p.edge1 = d + lead + p.clear_vecs * 16;
+    p.edge1_bytes = int(nbytes - lead - p.clear_vecs * 16);
+    // up to 16 clusters clear, 64 KiB a CTA at least
+    const unsigned clear = unsigned(std::min<long long>(16, 1 + p.clear_vecs / (kCsCtas * 2 * kCsClear)));
+    const dim3 grid(kCsCtas * (1 + clear));
+#define CYFA_CS(PER)                                                                             \
+  do {                                                                                           \
+    set_smem(embed_cluster_sort_kernel<PER>, cs_smem<PER>());                                    \
+    CYFA_LAUNCH("embed_sort", s, (launch_cluster_k(embed_cluster_sort_kernel<PER>, grid,         \
+                                                   kCsThreads, kCsCtas, cs_smem<PER>(), s, p))); \
+  } while (0)
+    const long long per = (N + kCsCtas * kCsThreads - 1) / (kCsCtas * kCsThreads);
+    if (per <= 1) CYFA_CS(1);
+    else if (per <= 2) CYFA_CS(2);
+    else if (per <= 4) CYFA_CS(4);
+    else if (per <= 8) CYFA_CS(8);
+    else CYFA_CS(16);
+#undef CYFA_CS
+  } else {
+    const cudaError_t e = cudaMemsetAsync(dweight, 0, size_t(V) * D * es, s);
+    if (e != cudaSuccess) return -static_cast<int>(e);
+    SortPass p{tokens, nullptr, nullptr, w.key[0], w.pos[0], w.count, N, V, padding_idx, 0,
+               int((N + kSortTile - 1) / kSortTile)};
+    for (int shift = 0; shift < 32 && (V >> shift) > 0; shift += 8) {
+      p.shift = shift;
+      CYFA_LAUNCH("embed_sort_count", s,
+                  (launch_k(embed_sort_count_kernel, unsigned(p.tiles), kSortThreads, 0, s, p)));
+      CYFA_LAUNCH("embed_sort_scan", s,
+                  (launch_k(embed_sort_scan_kernel, 1, 1024, 0, s, w.count, p.tiles * 256)));
+      CYFA_LAUNCH("embed_sort_move", s,
+                  (launch_k(embed_sort_move_kernel, unsigned(p.tiles), kSortThreads, 0, s, p)));
+      cur = p.key_out == w.key[0] ? 0 : 1;
+      p.tokens = nullptr;
+      p.key_in = w.key[cur];
+      p.pos_in = w.pos[cur];
+      p.key_out = w.key[1 - cur];
+      p.pos_out = w.pos[1 - cur];
+    }
   }
   EmbSumParams q{w.key[cur], w.pos[cur], dout, dweight, w.head, w.tail, N, uint32_t(V), D, scale};
   const int vec = embed_vec(D, es, dout, dweight);
@@ -401,11 +657,17 @@ int cyfa_embed_bwd(const long long* tokens, const void* dout, int dtype, void* d
   }
 #undef CYFA_EMB
   if (pieces > 1) {
-    const dim3 jgrid(pieces - 1, unsigned((D + 255) / 256));
-    if (dtype == 1)
-      CYFA_LAUNCH("embed_join", s, (launch_k(embed_join_kernel<__nv_bfloat16>, jgrid, 256, 0, s, q)));
-    else
-      CYFA_LAUNCH("embed_join", s, (launch_k(embed_join_kernel<float>, jgrid, 256, 0, s, q)));
+    // (a partial row starts at a multiple of 4 bytes D: float4 where D allows it)
+    const int jcols = D % 4 == 0 ? 128 : 32;
+    const dim3 jgrid(pieces - 1, unsigned(std::min((D + jcols - 1) / jcols, 8)));
+#define CYFA_EMB_JOIN(T, VEC) \
+  CYFA_LAUNCH("embed_join", s, (launch_k(embed_join_kernel<T, VEC>, jgrid, 256, 0, s, q)))
+    if (dtype == 1) {
+      if (D % 4 == 0) CYFA_EMB_JOIN(__nv_bfloat16, 4); else CYFA_EMB_JOIN(__nv_bfloat16, 1);
+    } else {
+      if (D % 4 == 0) CYFA_EMB_JOIN(float, 4); else CYFA_EMB_JOIN(float, 1);
+    }
+#undef CYFA_EMB_JOIN
   }
   return launch_status();
 }
