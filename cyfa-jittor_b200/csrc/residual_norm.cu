@@ -37,32 +37,34 @@ struct ResNormParams {
   int stages;                        // shared-memory slots of a streamed row: 2, or 1 (no copy ahead)
 };
 
-// A thread's 8 columns threadIdx.x + j blockDim.x of a row, for single elements.
-template <typename T>
+// A thread's 8 columns threadIdx.x + j TX of a row, for single elements (TX threads a
+// row, known to the compiler: the columns are then immediate offsets).
+template <typename T, int TX>
 struct RnRow {
   static constexpr int E = 8;
-  int off[E];
-  uint32_t mask;  // columns inside the row
-  __device__ __forceinline__ explicit RnRow(int D) : mask(0) {
+  int left;  // columns of the row from the thread's first on
+  __device__ __forceinline__ explicit RnRow(int D) : left(D - int(threadIdx.x)) {}
+  // p: the row, or null for zeros; n: left, or 0 for a row past the end
+  __device__ __forceinline__ void load(const T* p, int n, float (&f)[E]) const {
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      off[j] = int(threadIdx.x) + j * int(blockDim.x);
-      if (off[j] < D) mask |= 1u << j;
+    for (int j = 0; j < E; ++j) f[j] = 0.f;
+    if (p) {
+      p += threadIdx.x;
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (j * TX < n) f[j] = float(p[j * TX]);
     }
   }
-  // p: the row, or null for zeros
-  __device__ __forceinline__ void load(const T* p, uint32_t m, float (&f)[E]) const {
-#pragma unroll
-    for (int j = 0; j < E; ++j) f[j] = p && ((m >> j) & 1) ? float(p[off[j]]) : 0.f;
-  }
   __device__ __forceinline__ void param(const float* p, float (&f)[E]) const {
+    p += threadIdx.x;
 #pragma unroll
-    for (int j = 0; j < E; ++j) f[j] = (mask >> j) & 1 ? __ldg(p + off[j]) : 0.f;
+    for (int j = 0; j < E; ++j) f[j] = j * TX < left ? __ldg(p + j * TX) : 0.f;
   }
-  __device__ __forceinline__ void store(T* p, uint32_t m, const float (&f)[E]) const {
+  __device__ __forceinline__ void store(T* p, int n, const float (&f)[E]) const {
+    p += threadIdx.x;
 #pragma unroll
     for (int j = 0; j < E; ++j)
-      if ((m >> j) & 1) p[off[j]] = T(f[j]);
+      if (j * TX < n) p[j * TX] = T(f[j]);
   }
 };
 template <typename T>
@@ -86,12 +88,99 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   return s;
 }
 
+// Branch arithmetic.  A bf16 stream is normalised after it is rounded, so every error
+// of x' before that rounding moves some entries to the neighbouring bf16 value, 2^-8
+// off: with plain fp32 arithmetic one entry in 2^16, which is what then limits
+// dweight's distance from the exact sum (1e-5 relative).  For bf16 rows the branch is
+// therefore carried in pairs of fp32 numbers (value + error: 2^-29 with a gate, 2^-40
+// without), and x' is the exact sum's rounding but for one entry in 10^7 (16.7 M
+// entries: 0 or 1 off, against 220 to 560 of the plain formula).  fp32 rows use single
+// numbers.
+struct Pair {
+  float h, l;
+};
+__device__ __forceinline__ Pair pair_mul(Pair a, float b) {
+  const float h = a.h * b;
+  return Pair{h, fmaf(a.l, b, fmaf(a.h, b, -h))};
+}
+__device__ __forceinline__ Pair pair_mul(Pair a, Pair b) {
+  const float h = a.h * b.h;
+  return Pair{h, fmaf(a.h, b.l, fmaf(a.l, b.h, fmaf(a.h, b.h, -h)))};
+}
+// x + a, rounded once
+__device__ __forceinline__ float pair_add(float x, Pair a) {
+  const float s = x + a.h, b = s - x;
+  return s + (((x - (s - b)) + (a.h - b)) + a.l);
+}
+// 1 / (1 + e^-z).  e^-z = 2^k e^r with r = -z - k ln 2 in [-0.35, 0.35] (ln 2 split after
+// Cody and Waite, k ln2_hi exact) and e^r from its Taylor series, the terms up to
+// r^2 / 2 in pairs, the rest (below 2^-7) in fp32.
+__device__ __forceinline__ Pair pair_sigmoid(float z) {
+  const float a = fminf(fmaxf(-z, -87.f), 87.f);  // (NaN: any)
+  const float k = rintf(a * 1.44269504f);
+  // ln 2 = 45426 / 65536 + 1.4285946e-6 + rest
+  const float r0 = fmaf(-k, 0.693145751953125f, a);
+  const float p = k * 1.42860682e-6f;
+  const float rh = r0 - p, rl = (r0 - rh) - p;
+  const float qh = rh * rh, ql = fmaf(rh, rh, -qh) + 2.f * rh * rl;
+  // r^3 (1/6 + r/24 + r^2/120 + ... + r^7 / 10!)
+  float c = 2.7557319e-7f;
+  c = fmaf(c, rh, 2.7557319e-6f);
+  c = fmaf(c, rh, 2.4801587e-5f);
+  c = fmaf(c, rh, 1.9841270e-4f);
+  c = fmaf(c, rh, 1.3888889e-3f);
+  c = fmaf(c, rh, 8.3333333e-3f);
+  c = fmaf(c, rh, 4.1666667e-2f);
+  c = fmaf(c, rh, 1.6666667e-1f);
+  c *= qh * rh;
+  // e^r = 1 + r + r^2 / 2 + c as a pair
+  const float s1 = 1.f + rh, t1 = rh - (s1 - 1.f);
+  const float s2 = s1 + 0.5f * qh, t2 = 0.5f * qh - (s2 - s1);
+  const float s3 = s2 + c, t3 = c - (s3 - s2);
+  const float low = ((t1 + t2) + t3) + (rl + 0.5f * ql);
+  const float two_k = __int_as_float((int(k) + 127) << 23);
+  const float eh = s3 * two_k, el = low * two_k;
+  // 1 / (1 + e): a quotient and its remainder
+  const float d = 1.f + eh;
+  const float dl = (eh > 1.f ? (1.f - (d - eh)) : (eh - (d - 1.f))) + el;
+  const float g = __frcp_rn(d);
+  const float rem = fmaf(-dl, g, fmaf(-d, g, 1.f));
+  return z >= -87.f ? Pair{g, g * rem} : Pair{z != z ? z : 0.f, 0.f};
+}
+__device__ __forceinline__ float rn_gate(float z) { return 1.f / (1.f + expf(-z)); }
+
+// Sum of squares of bf16 values (exact products), as a pair.
+__device__ __forceinline__ void pair_square(float y, float& s, float& c) {
+  const float q = y * y, t = s + q, b = t - s;
+  c += (s - (t - b)) + (q - b);
+  s = t;
+}
+// row_sum of pairs, in 64 bits
+__device__ __forceinline__ double row_sum_pair(float s, float c, double* red) {
+  double v = double(s) + double(c);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int warps = int(blockDim.x) >> 5;
+  if (warps == 1) return v;
+  red += threadIdx.y * warps;
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.0;
+  for (int w = 0; w < warps; ++w) v += red[w];
+  return v;
+}
+__device__ __forceinline__ Pair pair_of(double v) {
+  const float h = float(v);
+  return Pair{h, float(v - double(h))};
+}
+
 template <typename T>
 __device__ __forceinline__ float rn_round(float v) {
   return float(T(v));
 }
 
-// ------------------------------------------------ rows of 16-byte vectors
+// ------------------------------------------------ streamed rows
 // Persistent CTAs of blockDim (threads of a row, rows at a time).  Each thread copies
 // its E columns of the next row into its own shared-memory slots (cp.async, no
 // barrier: nobody else reads them) while it works on the current one, so that the
@@ -148,6 +237,7 @@ __global__ void __launch_bounds__(256) residual_norm_fwd_stream_kernel(ResNormPa
   constexpr int VEC = S::VEC, J = S::J;
   extern __shared__ __align__(16) uint8_t rn_smem[];
   __shared__ float red[32];
+  __shared__ double red64[32];
   pdl_wait();
   pdl_trigger();
   const int D = p.D;
@@ -170,17 +260,26 @@ __global__ void __launch_bounds__(256) residual_norm_fwd_stream_kernel(ResNormPa
     const bool first = row < p.rows && threadIdx.x == 0;
     T* xn = static_cast<T*>(p.xn) + row * D + st.c0;
     T* h = static_cast<T*>(p.h) + row * D + st.c0;
+    constexpr bool PAIRS = sizeof(T) == 2;
     float rsy = 1.f;
+    Pair rsp{1.f, 0.f};
     if (!PLAIN && p.post) {
-      float ss = 0.f;
+      float ss = 0.f, sc = 0.f;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         float y[VEC];
         st.get(s, 1, j, y);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) ss = fmaf(y[i], y[i], ss);
+        for (int i = 0; i < VEC; ++i) {
+          if (PAIRS) pair_square(y[i], ss, sc); else ss = fmaf(y[i], y[i], ss);
+        }
       }
-      rsy = rsqrtf(row_sum(ss, red) / D + p.eps);
+      if (PAIRS) {
+        rsp = pair_of(1.0 / sqrt(row_sum_pair(ss, sc, red64) / D + double(p.eps)));
+        rsy = rsp.h;
+      } else {
+        rsy = __frsqrt_rn(row_sum(ss, red) / D + p.eps);
+      }
       if (first && p.rstd_y) p.rstd_y[row] = rsy;
     }
     float ss = 0.f;
@@ -191,29 +290,30 @@ __global__ void __launch_bounds__(256) residual_norm_fwd_stream_kernel(ResNormPa
       if (PLAIN || p.y) {
         float z[VEC];
         st.get(s, 1, j, z);
-        if (!PLAIN) {
-          float f[VEC];
-          if (p.post) {
-            st.param(p.post, j, f);
+        if (PLAIN) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) z[i] = z[i] * rsy * f[i];
-          }
-          if (p.gate) {
-            st.get(s, 2, j, f);
+          for (int i = 0; i < VEC; ++i) t[i] += z[i];
+        } else {
+          float w[VEC], g[VEC], sc[VEC];
+          if (p.post) st.param(p.post, j, w);
+          if (p.gate) st.get(s, 2, j, g);
+          if (p.scale_v) st.param(p.scale_v, j, sc);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) z[i] *= sigmoid_mufu(f[i]);
-          }
-          if (p.scale_v) {
-            st.param(p.scale_v, j, f);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) z[i] *= f[i];
-          } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) z[i] *= p.scale;
+          for (int i = 0; i < VEC; ++i) {
+            const float scale = p.scale_v ? sc[i] : p.scale;
+            if (PAIRS) {
+              Pair u{z[i], 0.f};
+              if (p.post) u = pair_mul(pair_mul(rsp, z[i]), w[i]);
+              if (p.gate) u = pair_mul(u, pair_sigmoid(g[i]));
+              t[i] = pair_add(t[i], pair_mul(u, scale));
+            } else {
+              float u = z[i];
+              if (p.post) u = u * rsy * w[i];
+              if (p.gate) u *= rn_gate(g[i]);
+              t[i] = fmaf(scale, u, t[i]);
+            }
           }
         }
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) t[i] += z[i];
         // the norm reads the stream as it is kept, in x's type
         const uint4 u = LpVec<T>::pack(t);
         LpVec<T>::unpack(u, t);
@@ -223,7 +323,7 @@ __global__ void __launch_bounds__(256) residual_norm_fwd_stream_kernel(ResNormPa
 #pragma unroll
       for (int i = 0; i < VEC; ++i) ss = fmaf(t[i], t[i], ss);
     }
-    const float rs = rsqrtf(row_sum(ss, red) / D + p.eps);
+    const float rs = __frsqrt_rn(row_sum(ss, red) / D + p.eps);
     if (first && p.rstd_x) p.rstd_x[row] = rs;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
@@ -394,61 +494,72 @@ __global__ void __launch_bounds__(256) residual_norm_bwd_stream_kernel(ResNormPa
 }
 
 // ------------------------------------------------ rows at any alignment
-// Persistent CTAs as above, all of a row's loads ahead of its sums.
-template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) residual_norm_fwd_kernel(ResNormParams p) {
-  using R = RnRow<T>;
+// Persistent CTAs as above, a thread's 8 columns TX apart, all of a row's loads ahead
+// of its sums.  What bounds these is the issue of one access an element; 4-byte
+// asynchronous copies into shared memory in their place took 55 and 126 us (forward
+// and backward, 4099 x 1531 fp32 with both norms, gate and scale).
+template <typename T, int TX>
+__global__ void __launch_bounds__(TX > 256 ? TX : 256, TX > 256 ? 1 : 4)
+    residual_norm_fwd_kernel(ResNormParams p) {
+  using R = RnRow<T, TX>;
   constexpr int E = R::E;
   pdl_wait();
   pdl_trigger();
   __shared__ float red[32];
+  __shared__ double red64[32];
   const int D = p.D;
   const R r(D);
   for (long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y; row - threadIdx.y < p.rows;
        row += (long long)gridDim.x * blockDim.y) {
     // rows past the end take part in the barriers only
-    const uint32_t m = row < p.rows ? r.mask : 0;
+    const int m = row < p.rows ? r.left : 0;
     const bool first = row < p.rows && threadIdx.x == 0;
     float t[E], z[E], g[E];
     r.load(rn_at<T>(p.x, row * p.sx), m, t);
     r.load(rn_at<T>(p.y, row * p.sy), m, z);
     r.load(rn_at<T>(p.gate, row * p.sgate), m, g);
     if (p.y) {
-      if (p.gate) {
-#pragma unroll
-        for (int i = 0; i < E; ++i) g[i] = sigmoid_mufu(g[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i) g[i] = 1.f;
-      }
-      float w[E];
+      constexpr bool PAIRS = sizeof(T) == 2;
+      float w[E], sv[E], rsy = 1.f;
+      Pair rsp{1.f, 0.f};
       if (p.post) {
-        float ss = 0.f;
+        float ss = 0.f, sc = 0.f;
 #pragma unroll
-        for (int i = 0; i < E; ++i) ss = fmaf(z[i], z[i], ss);
-        const float rs = rsqrtf(row_sum(ss, red) / D + p.eps);
+        for (int i = 0; i < E; ++i) {
+          if (PAIRS) pair_square(z[i], ss, sc); else ss = fmaf(z[i], z[i], ss);
+        }
+        if (PAIRS) {
+          rsp = pair_of(1.0 / sqrt(row_sum_pair(ss, sc, red64) / D + double(p.eps)));
+          rsy = rsp.h;
+        } else {
+          rsy = __frsqrt_rn(row_sum(ss, red) / D + p.eps);
+        }
         r.param(p.post, w);
-#pragma unroll
-        for (int i = 0; i < E; ++i) z[i] = z[i] * rs * w[i];
-        if (first && p.rstd_y) p.rstd_y[row] = rs;
+        if (first && p.rstd_y) p.rstd_y[row] = rsy;
       }
-      if (p.scale_v) {
-        r.param(p.scale_v, w);
+      if (p.scale_v) r.param(p.scale_v, sv);
 #pragma unroll
-        for (int i = 0; i < E; ++i) g[i] *= w[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i) g[i] *= p.scale;
+      for (int i = 0; i < E; ++i) {
+        const float scale = p.scale_v ? sv[i] : p.scale;
+        if (PAIRS) {
+          Pair u{z[i], 0.f};
+          if (p.post) u = pair_mul(pair_mul(rsp, z[i]), w[i]);
+          if (p.gate) u = pair_mul(u, pair_sigmoid(g[i]));
+          t[i] = pair_add(t[i], pair_mul(u, scale));
+        } else {
+          float u = z[i];
+          if (p.post) u = u * rsy * w[i];
+          if (p.gate) u *= rn_gate(g[i]);
+          t[i] = fmaf(scale, u, t[i]);
+        }
+        t[i] = rn_round<T>(t[i]);  // the norm reads the stream as it is kept, in x's type
       }
-      // the norm reads the stream as it is kept, in x's type
-#pragma unroll
-      for (int i = 0; i < E; ++i) t[i] = rn_round<T>(fmaf(g[i], z[i], t[i]));
       r.store(static_cast<T*>(p.xn) + row * D, m, t);
     }
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < E; ++i) ss = fmaf(t[i], t[i], ss);
-    const float rs = rsqrtf(row_sum(ss, red) / D + p.eps);
+    const float rs = __frsqrt_rn(row_sum(ss, red) / D + p.eps);
     if (first && p.rstd_x) p.rstd_x[row] = rs;
     r.param(p.weight, g);
 #pragma unroll
@@ -458,9 +569,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) residual_norm_fwd_ker
 }
 
 // p.x is the new stream x'.
-template <typename T, int THREADS, bool FULL>
-__global__ void __launch_bounds__(THREADS) residual_norm_bwd_kernel(ResNormParams p) {
-  using R = RnRow<T>;
+template <typename T, int TX, bool FULL>
+__global__ void __launch_bounds__(TX > 256 ? TX : 256, TX > 256 ? 1 : (FULL ? 2 : 3))
+    residual_norm_bwd_kernel(ResNormParams p) {
+  using R = RnRow<T, TX>;
   constexpr int E = R::E;
   extern __shared__ __align__(16) uint8_t rn_smem[];
   __shared__ float red[32];
@@ -477,7 +589,7 @@ __global__ void __launch_bounds__(THREADS) residual_norm_bwd_kernel(ResNormParam
   for (long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y; row - threadIdx.y < p.rows;
        row += (long long)gridDim.x * blockDim.y) {
     const bool in = row < p.rows;
-    const uint32_t m = in ? r.mask : 0;
+    const int m = in ? r.left : 0;
     float t[E], g[E], dt[E], y[E], sg[E], w[E];
     r.load(rn_at<T>(p.x, row * p.sx), m, t);
     r.load(rn_at<T>(p.dh, row * D), m, g);
@@ -547,7 +659,7 @@ __global__ void __launch_bounds__(THREADS) residual_norm_bwd_kernel(ResNormParam
                            [&](int k, float* row_buf) {
 #pragma unroll
                              for (int j = 0; j < E; ++j)
-                               if ((r.mask >> j) & 1) row_buf[r.off[j]] = acc[k][j];
+                               if (j * TX < r.left) row_buf[threadIdx.x + j * TX] = acc[k][j];
                            });
 }
 
@@ -574,18 +686,23 @@ __global__ void __launch_bounds__(1024)
   if (threadIdx.x == 0 && cc < D) out[cc] = v;
 }
 
+// Columns of a thread: 8; with 16-byte accesses 32 once 8 would be more than a warp a
+// row (8192 columns are 256 threads), and 16 with y's side up to 4096 columns, for
+// the three accumulators a column.
+static int rn_elems(int D, bool vector, bool full) {
+  return !vector || D <= 256 ? 8 : (full && D <= 4096 ? 16 : 32);
+}
 // threads of a row with E columns each, and rows of a CTA
-static dim3 rn_block(int D, int E, long long rows) {
-  const int tx = ((D + E - 1) / E + 31) / 32 * 32;
+static dim3 rn_block(int D, int E, bool vector, long long rows) {
+  int tx = ((D + E - 1) / E + 31) / 32 * 32;
+  if (!vector) {  // the spacings that are built
+    int t = 32;
+    while (t < tx) t = t == 256 ? 1024 : 2 * t;
+    tx = t;
+  }
   int ty = 1;
   while (ty < 8 && tx * ty * 2 <= 256 && rows > ty) ty *= 2;
   return dim3(unsigned(tx), unsigned(ty));
-}
-// Columns of a thread: 8, or 32 with 16-byte accesses once 8 would be more than a warp
-// a row (8192 columns are 256 threads); with y's side 16-byte accesses keep 16, for
-// the three accumulators a column.
-static int rn_elems(int D, int vec, bool full) {
-  return vec == 1 || D <= 256 ? 8 : (full && D <= 4096 ? 16 : 32);
 }
 // shared memory of one slot of a row's tensors; two slots where they fit (they do not
 // for four or five fp32 tensors of more than 5600 columns)
@@ -595,9 +712,9 @@ static size_t rn_slot_bytes(dim3 block, int elems, int es, int tensors) {
 constexpr int kRnMaxSmem = 226 << 10;
 static int rn_stages(size_t slot) { return 2 * slot <= kRnMaxSmem ? 2 : 1; }
 // CTAs an SM holds at a time (shared memory and registers)
-static int rn_per_sm(dim3 block, int vec, size_t smem) {
+static int rn_per_sm(dim3 block, bool vector, size_t smem) {
   const int threads = int(block.x * block.y);
-  if (vec == 1) return std::max(1, 1024 / threads);
+  if (!vector) return std::max(1, 1024 / threads);
   return int(std::max<size_t>(1, std::min<size_t>(std::min<size_t>(4, 768 / threads),
                                                   (220 << 10) / (smem + 1024))));
 }
@@ -606,27 +723,26 @@ struct RnBwdShape {
   dim3 block;
   size_t smem;
   unsigned grid;
-  RnBwdShape(int D, int es, long long rows, bool full, bool gate, int vec) {
-    elems = rn_elems(D, vec, full);
-    block = rn_block(D, elems, rows);
+  RnBwdShape(int D, int es, long long rows, bool full, bool gate, bool vector) {
+    elems = rn_elems(D, vector, full);
+    block = rn_block(D, elems, vector, rows);
     const size_t slot = rn_slot_bytes(block, elems, es, full ? 4 + gate : 3);
     stages = rn_stages(slot);
-    smem = vec == 1 ? block.y * D * sizeof(float) : stages * slot;
+    smem = vector ? stages * slot : block.y * D * sizeof(float);
     grid = unsigned(std::min<long long>((rows + block.y - 1) / block.y,
-                                        148ll * rn_per_sm(block, vec, smem)));
+                                        148ll * rn_per_sm(block, vector, smem)));
   }
 };
 
-// 16-byte accesses where every row and parameter allows them, else single elements
-static int rn_vec(int D, int es, std::initializer_list<const void*> ptrs,
-                  std::initializer_list<const float*> params,
-                  std::initializer_list<long long> strides) {
-  const int vec = 16 / es;
-  bool ok = D % vec == 0;
+// Whether every row and parameter allows 16-byte accesses.
+static bool rn_vector(int D, int es, std::initializer_list<const void*> ptrs,
+                      std::initializer_list<const float*> params,
+                      std::initializer_list<long long> strides) {
+  bool ok = D * es % 16 == 0;
   for (const void* q : ptrs) ok = ok && aligned(q, 16);
   for (const float* q : params) ok = ok && aligned(q, 16);
-  for (long long st : strides) ok = ok && st % vec == 0;
-  return ok ? vec : 1;
+  for (long long st : strides) ok = ok && st * es % 16 == 0;
+  return ok;
 }
 
 static int rn_checks(int dtype, long long rows, int D) {
@@ -667,17 +783,18 @@ int cyfa_residual_norm_fwd(const cyfa_residual_norm_args* a, void* xn, void* h, 
   p.h = h;
   p.rstd_x = rstd_x;
   p.rstd_y = rstd_y;
-  const int vec = rn_vec(a->D, es, {a->x, a->y, a->gate, xn, h}, {a->weight, a->post_weight, a->scale_vector},
-                         {a->x_stride, a->y ? a->y_stride : 0, a->gate ? a->gate_stride : 0});
-  const int elems = rn_elems(a->D, vec, false);
-  const dim3 block = rn_block(a->D, elems, a->rows);
+  const bool vector = rn_vector(a->D, es, {a->x, a->y, a->gate, xn, h},
+                                {a->weight, a->post_weight, a->scale_vector},
+                                {a->x_stride, a->y ? a->y_stride : 0, a->gate ? a->gate_stride : 0});
+  const int elems = rn_elems(a->D, vector, false);
+  const dim3 block = rn_block(a->D, elems, vector, a->rows);
   const long long ctas = (a->rows + block.y - 1) / block.y;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (vec > 1) {
+  if (vector) {
     const size_t slot = rn_slot_bytes(block, elems, es, 1 + (a->y != nullptr) + (a->gate != nullptr));
     p.stages = rn_stages(slot);
     const size_t smem = p.stages * slot;
-    const unsigned grid = unsigned(std::min<long long>(ctas, 148ll * rn_per_sm(block, vec, smem)));
+    const unsigned grid = unsigned(std::min<long long>(ctas, 148ll * rn_per_sm(block, vector, smem)));
     const bool plain = a->y && !a->post_weight && !a->gate && !a->scale_vector && a->scale == 1.f;
 #define CYFA_RN_L(T, E, PLAIN)                                                                       \
   do {                                                                                               \
@@ -696,15 +813,21 @@ int cyfa_residual_norm_fwd(const cyfa_residual_norm_args* a, void* xn, void* h, 
 #undef CYFA_RN_L
     return launch_status();
   }
-#define CYFA_RN(T, THREADS)            \
+  const unsigned grid = unsigned(std::min<long long>(ctas, 148ll * rn_per_sm(block, vector, 0)));
+#define CYFA_RN_L(T, TX)               \
   CYFA_LAUNCH("residual_norm_fwd", s, \
-              (launch_k(residual_norm_fwd_kernel<T, THREADS>, unsigned(std::min<long long>(ctas, 148 * rn_per_sm(block, 1, 0))), block, 0, s, p)))
-  if (a->dtype == 1) {
-    if (block.x > 256) CYFA_RN(__nv_bfloat16, 1024); else CYFA_RN(__nv_bfloat16, 256);
-  } else {
-    if (block.x > 256) CYFA_RN(float, 1024); else CYFA_RN(float, 256);
-  }
+              (launch_k(residual_norm_fwd_kernel<T, TX>, grid, block, 0, s, p)))
+#define CYFA_RN(T)                              \
+  do {                                          \
+    if (block.x == 32) CYFA_RN_L(T, 32);        \
+    else if (block.x == 64) CYFA_RN_L(T, 64);   \
+    else if (block.x == 128) CYFA_RN_L(T, 128); \
+    else if (block.x == 256) CYFA_RN_L(T, 256); \
+    else CYFA_RN_L(T, 1024);                    \
+  } while (0)
+  if (a->dtype == 1) CYFA_RN(__nv_bfloat16); else CYFA_RN(float);
 #undef CYFA_RN
+#undef CYFA_RN_L
   return launch_status();
 }
 
@@ -712,7 +835,7 @@ size_t cyfa_residual_norm_bwd_work_bytes(long long rows, int D) {
   if (rows <= 0 || D <= 0 || D > kRnMaxWidth) return 0;
   size_t most = 0;
   for (int k = 0; k < 16; ++k) {
-    const RnBwdShape sh(D, k & 1 ? 2 : 4, rows, k & 2, k & 4, k & 8 ? 4 : 1);
+    const RnBwdShape sh(D, k & 1 ? 2 : 4, rows, k & 2, k & 4, k & 8);
     most = std::max(most, size_t(sh.grid));
   }
   return most * 3 * D * sizeof(float);
@@ -757,10 +880,10 @@ int cyfa_residual_norm_bwd(const cyfa_residual_norm_args* a, const float* rstd_x
   p.part = static_cast<float*>(work);
   // without gate, scale and post-norm, dy equals dx: the plain sum's gradient
   const bool full = a->y && (dy || dgate || dpost || dscale);
-  const int vec = rn_vec(a->D, es, {a->x, a->y, a->gate, dxn, dh, dx, dy, dgate},
-                         {a->weight, a->post_weight, a->scale_vector},
-                         {a->x_stride, a->y ? a->y_stride : 0, a->gate ? a->gate_stride : 0});
-  const RnBwdShape sh(a->D, es, a->rows, full, a->gate != nullptr, vec);
+  const bool vector = rn_vector(a->D, es, {a->x, a->y, a->gate, dxn, dh, dx, dy, dgate},
+                                {a->weight, a->post_weight, a->scale_vector},
+                                {a->x_stride, a->y ? a->y_stride : 0, a->gate ? a->gate_stride : 0});
+  const RnBwdShape sh(a->D, es, a->rows, full, a->gate != nullptr, vector);
   p.stages = sh.stages;
   const dim3 block = sh.block;
   const unsigned grid = sh.grid;
@@ -771,16 +894,19 @@ int cyfa_residual_norm_bwd(const cyfa_residual_norm_args* a, const float* rstd_x
     CYFA_LAUNCH("residual_norm_bwd", s,                                                              \
                 (launch_k(residual_norm_bwd_stream_kernel<T, E, FULL>, grid, block, sh.smem, s, p))); \
   } while (0)
-#define CYFA_RN_L(T, THREADS, FULL)    \
+#define CYFA_RN_L(T, TX, FULL)         \
   CYFA_LAUNCH("residual_norm_bwd", s, \
-              (launch_k(residual_norm_bwd_kernel<T, THREADS, FULL>, grid, block, sh.smem, s, p)))
-#define CYFA_RN(T, FULL)                                        \
-  do {                                                          \
-    if (vec > 1 && sh.elems == 8) CYFA_RN_S(T, 8, FULL);        \
-    else if (vec > 1 && sh.elems == 16) CYFA_RN_S(T, 16, FULL); \
-    else if (vec > 1) CYFA_RN_S(T, 32, FULL);                   \
-    else if (block.x > 256) CYFA_RN_L(T, 1024, FULL);           \
-    else CYFA_RN_L(T, 256, FULL);                               \
+              (launch_k(residual_norm_bwd_kernel<T, TX, FULL>, grid, block, sh.smem, s, p)))
+#define CYFA_RN(T, FULL)                                          \
+  do {                                                            \
+    if (vector && sh.elems == 8) CYFA_RN_S(T, 8, FULL);           \
+    else if (vector && sh.elems == 16) CYFA_RN_S(T, 16, FULL);    \
+    else if (vector) CYFA_RN_S(T, 32, FULL);                      \
+    else if (block.x == 32) CYFA_RN_L(T, 32, FULL);               \
+    else if (block.x == 64) CYFA_RN_L(T, 64, FULL);               \
+    else if (block.x == 128) CYFA_RN_L(T, 128, FULL);             \
+    else if (block.x == 256) CYFA_RN_L(T, 256, FULL);             \
+    else CYFA_RN_L(T, 1024, FULL);                                \
   } while (0)
   if (a->dtype == 1) {
     if (full) CYFA_RN(__nv_bfloat16, true); else CYFA_RN(__nv_bfloat16, false);
