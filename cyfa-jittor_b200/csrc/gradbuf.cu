@@ -169,6 +169,66 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
   }
 }
 
+// ---------------------------------------------------------------- Muon
+// The element-wise halves of a Muon step around the orthogonalisation of its
+// matrices (cyfa_newton_schulz), over the same flat buffers:
+//   m = mu m + g,  u = g + mu m (Nesterov) or m        -> u, one dense matrix a piece
+//   master = master (1 - lr decay) - step_size o       (o: the orthogonalised u, bf16)
+// Bound by bandwidth: 16 bytes an element each.
+struct MuonArgs {
+  BucketArgs pieces;  // momentum: ptr = u (f32); apply: ptr = the parameters
+  float* m;           // momentum
+  const float* grad;
+  float* master;      // apply
+  const __nv_bfloat16* update[kMaxPieces];
+  float mu, shrink, step_size;
+  int nesterov;
+};
+
+template <bool APPLY>
+__global__ void __launch_bounds__(256) muon_kernel(const __grid_constant__ MuonArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  const BucketArgs& pc = a.pieces;
+  const int i = bucket_piece(pc, blockIdx.x);
+  const long long e0 = (long long)(blockIdx.x - pc.blk_prefix[i]) * kBucketChunk + threadIdx.x * 8;
+  const long long n = pc.n[i];
+  if (e0 >= n) return;
+  const long long f = pc.off[i] + e0;
+  const int cnt = n - e0 < 8 ? int(n - e0) : 8;
+  float v[8];
+  if (APPLY) {
+    const __nv_bfloat16* o = a.update[i] + e0;
+    float u[8];
+    if (cnt == 8 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+      unpack_bf16x8(*reinterpret_cast<const uint4*>(o), u);
+    } else {
+      for (int k = 0; k < cnt; ++k) u[k] = __bfloat162float(o[k]);
+    }
+    for (int k = 0; k < cnt; ++k) v[k] = a.master[f + k] * a.shrink - a.step_size * u[k];
+    for (int k = 0; k < cnt; ++k) a.master[f + k] = v[k];
+    if (pc.dtype[i] == 1) {
+      __nv_bfloat16* w = static_cast<__nv_bfloat16*>(pc.ptr[i]) + e0;
+      if (cnt == 8) {
+        *reinterpret_cast<uint4*>(w) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]),
+                                                  pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+      } else {
+        for (int k = 0; k < cnt; ++k) w[k] = __float2bfloat16_rn(v[k]);
+      }
+    } else {
+      float* w = static_cast<float*>(pc.ptr[i]) + e0;
+      for (int k = 0; k < cnt; ++k) w[k] = v[k];
+    }
+  } else {
+    float* u = static_cast<float*>(pc.ptr[i]) + e0;
+    for (int k = 0; k < cnt; ++k) {
+      const float g = a.grad[f + k], m = fmaf(a.mu, a.m[f + k], g);
+      a.m[f + k] = m;
+      u[k] = a.nesterov ? fmaf(a.mu, m, g) : m;
+    }
+  }
+}
+
 // ---------------------------------------------------------------- gradient clipping
 // L2 norm of a flat fp32 gradient buffer in a fixed order (per-block partial sums
 // of squares, then one block sums them), the clip coefficient
@@ -311,6 +371,80 @@ int cyfa_adamw_step(const cyfa_bucket_piece* params, int count, float* master, f
     CYFA_LAUNCH("adamw", st, (launch_k(adamw_kernel, unsigned(blocks), 256, 0, st, a)));
     const int rc = launch_status();
     if (rc != kOk) return rc;
+  }
+  return kOk;
+}
+
+}  // extern "C"
+
+// Fills pieces [base, ...) of a Muon call; the block count in `blocks`.
+static int muon_pieces(MuonArgs& a, const cyfa_bucket_piece* pieces, const void* const* updates,
+                       int base, int count, long long& blocks) {
+  BucketArgs& pc = a.pieces;
+  pc.count = count - base < kMaxPieces ? count - base : kMaxPieces;
+  blocks = 0;
+  for (int i = 0; i < pc.count; ++i) {
+    const cyfa_bucket_piece& p = pieces[base + i];
+    CYFA_REQUIRE(p.n > 0 && p.offset >= 0, kBadShape);
+    CYFA_REQUIRE(p.dtype == 0 || (updates && p.dtype == 1), kBadDtype);
+    CYFA_REQUIRE(p.ptr && (!updates || updates[base + i]), kNullPointer);
+    CYFA_REQUIRE(aligned(p.ptr, updates ? 16 : 4) && p.offset % 8 == 0 &&
+                     (!updates || aligned(updates[base + i], 2)),
+                 kMisaligned);
+    pc.blk_prefix[i] = static_cast<int>(blocks);
+    pc.ptr[i] = p.ptr;
+    pc.n[i] = p.n;
+    pc.off[i] = p.offset;
+    pc.dtype[i] = p.dtype;
+    if (updates) a.update[i] = static_cast<const __nv_bfloat16*>(updates[base + i]);
+    blocks += (p.n + kBucketChunk - 1) / kBucketChunk;
+    CYFA_REQUIRE(blocks < (1LL << 30), kBadShape);
+  }
+  pc.blk_prefix[pc.count] = static_cast<int>(blocks);
+  return kOk;
+}
+
+extern "C" {
+
+int cyfa_muon_momentum(const cyfa_bucket_piece* pieces, int count, float* m, const float* grad,
+                       float momentum, int nesterov, void* stream) {
+  CYFA_REQUIRE(count >= 0, kBadShape);
+  CYFA_REQUIRE(count == 0 || (pieces && m && grad), kNullPointer);
+  CYFA_REQUIRE(aligned(m, 16) && aligned(grad, 16), kMisaligned);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  for (int base = 0; base < count; base += kMaxPieces) {
+    MuonArgs a{};
+    long long blocks;
+    int rc = muon_pieces(a, pieces, nullptr, base, count, blocks);
+    if (rc) return rc;
+    a.m = m;
+    a.grad = grad;
+    a.mu = momentum;
+    a.nesterov = nesterov;
+    CYFA_LAUNCH("muon_momentum", st, (launch_k(muon_kernel<false>, unsigned(blocks), 256, 0, st, a)));
+    rc = launch_status();
+    if (rc) return rc;
+  }
+  return kOk;
+}
+
+int cyfa_muon_apply(const cyfa_bucket_piece* params, const void* const* updates, int count,
+                    float* master, float step_size, float shrink, void* stream) {
+  CYFA_REQUIRE(count >= 0, kBadShape);
+  CYFA_REQUIRE(count == 0 || (params && updates && master), kNullPointer);
+  CYFA_REQUIRE(aligned(master, 16), kMisaligned);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  for (int base = 0; base < count; base += kMaxPieces) {
+    MuonArgs a{};
+    long long blocks;
+    int rc = muon_pieces(a, params, updates, base, count, blocks);
+    if (rc) return rc;
+    a.master = master;
+    a.step_size = step_size;
+    a.shrink = shrink;
+    CYFA_LAUNCH("muon_apply", st, (launch_k(muon_kernel<true>, unsigned(blocks), 256, 0, st, a)));
+    rc = launch_status();
+    if (rc) return rc;
   }
   return kOk;
 }

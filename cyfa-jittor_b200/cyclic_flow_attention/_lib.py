@@ -65,6 +65,8 @@ _SIGNATURES = {
     "cyfa_embed_bwd": [_vp, _vp, _i, _vp, _ll, _ll, _i, _f, _ll, _vp, ctypes.c_size_t, _vp],
     "cyfa_residual_norm_fwd": [_vp] * 6,
     "cyfa_residual_norm_bwd": [_vp] * 12 + [ctypes.c_size_t, _vp],
+    "cyfa_muon_momentum": [_vp, _i, _vp, _vp, _f, _i, _vp],
+    "cyfa_muon_apply": [_vp, _vp, _i, _vp, _f, _f, _vp],
     "cyfa_newton_schulz": [_vp] + [_i] * 5 + [_f] * 4 + [_vp, _vp, ctypes.c_size_t, _vp],
 }
 

@@ -11,6 +11,8 @@ round trip.
 
 import torch
 
+from .ops.token_ops import token_log_probs
+
 
 def _validate(ids, max_new_tokens, temperature=0.0, top_p=1.0):
     if not ids or max_new_tokens < 0 or temperature < 0 or not 0 < top_p <= 1:
@@ -97,19 +99,28 @@ class GraphedDecoder:
     returns the prompt's n greedy continuation tokens [B, n] on the device.
     The captured graph holds the cache tensors' addresses: a new prefill
     captures a new graph.
+
+    With ``top`` given (0 for none), the step also rates its choice:
+    ``scores`` holds the log probability [B] of the token just returned, the
+    entropy of its distribution and the ``top`` alternatives
+    (``ops.TokenLogProbs``), overwritten by the next step.
     """
 
-    def __init__(self, model):
+    def __init__(self, model, top=None):
         self.model = model.eval()
         self.graph = None
+        self.top = top
+        self.scores = None
 
     @torch.no_grad()
     def prefill(self, input_ids):
         m = self.model
         self.graph = None
         hidden, cache = m.model(input_ids, use_cache=True)
-        first = m.lm_head(hidden[:, -1]).argmax(-1, keepdim=True)
-        del hidden
+        logits = m.lm_head(hidden[:, -1])
+        first = logits.argmax(-1, keepdim=True)
+        first_scores = self._rate(logits, first)
+        del hidden, logits
         for c in cache:
             c["conv_state"] = tuple(t.contiguous() for t in c["conv_state"])
             c["recurrent_state"] = tuple(t.contiguous() for t in c["recurrent_state"])
@@ -125,11 +136,17 @@ class GraphedDecoder:
         with torch.cuda.graph(self.graph):
             logits, _ = m.decode_step(self.ids, self.cache, inplace=True)
             self.ids.copy_(logits.argmax(-1, keepdim=True))
+            self._step_scores = self._rate(logits, self.ids)
+        self.scores = first_scores
         return first
+
+    def _rate(self, logits, ids):
+        return None if self.top is None else token_log_probs(logits, ids[:, 0], top=self.top)
 
     def step(self):
         """Consumes the current token of every row, returns the next [B, 1]."""
         self.graph.replay()
+        self.scores = self._step_scores
         return self.ids
 
     @torch.no_grad()

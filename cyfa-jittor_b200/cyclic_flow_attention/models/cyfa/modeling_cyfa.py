@@ -6,11 +6,16 @@ module tree and parameter names (``model.embeddings``, ``model.layers.N.attn``,
 ``lm_head``), so the reference's safetensors checkpoints load unchanged
 (``cyclic_flow_attention.utils.load_model``).
 
-Two execution paths:
+Execution paths:
 * ``forward`` over a sequence: with gradients (training) the attention layer's
   fused path with the block norms and the gated MLP in PyTorch as the reference
   computes them (fp32 math, bf16 results); without (prefill) the same glue
   launches as the decode step below.
+* ``forward`` with gradients after ``fuse_training()``: the embedding
+  (``embed_tokens``), every residual add with the norm that follows it
+  (``residual_norm``) and the loss (``token_log_probs``) as libcyfa operators with
+  their own gradients, the same values up to the rounding of fp32 sums.
+* ``score``: log probabilities of a text's tokens, with entropies and alternatives.
 * ``decode_step`` for one token per sequence with a cache: every piece of glue
   is one libcyfa launch (``cyfa_add_rmsnorm`` for residual + norm,
   ``cyfa_swiglu`` for the MLP activation) around cuBLAS GEMMs on packed
@@ -28,6 +33,8 @@ from torch import nn
 from ... import _lib
 from ...layers.cyfa import CyclicFlowAttention, RMSNorm
 from ...ops.layer_ops import packed_rows
+from ...ops.norm_ops import MAX_WIDTH, residual_norm
+from ...ops.token_ops import embed_tokens, token_log_probs
 from .configuration_cyfa import CyclicFlowAttentionConfig
 
 # Parameters the reference keeps in fp32 when it casts a model to bf16
@@ -117,6 +124,12 @@ class CyclicFlowAttentionModel(nn.Module):
         self.embeddings = nn.Embedding(config.vocab_size, config.hidden_size)
         self.layers = nn.ModuleList([CyFABlock(config) for _ in range(config.num_hidden_layers)])
         self.norm = RMSNorm(config.hidden_size, config.norm_eps)
+        self.fused_training = False
+
+    def _train_ops_ok(self, input_ids):
+        w = self.embeddings.weight
+        return (self.fused_training and torch.is_grad_enabled() and w.is_cuda
+                and w.dtype == torch.bfloat16 and input_ids.is_cuda and w.shape[1] <= MAX_WIDTH)
 
     def _glue_ok(self, input_ids):
         w = self.embeddings.weight
@@ -128,12 +141,28 @@ class CyclicFlowAttentionModel(nn.Module):
     def forward(self, input_ids, cache=None, use_cache=False, attention_mask=None):
         if self._glue_ok(input_ids):
             return self._forward_glue(input_ids, cache, use_cache, attention_mask)
+        if self._train_ops_ok(input_ids):
+            return self._forward_train(input_ids, cache, use_cache, attention_mask)
         x = self.embeddings(input_ids)
         new = []
         for i, layer in enumerate(self.layers):
             x, s = layer(x, None if cache is None else cache[i], use_cache, attention_mask)
             new.append(s)
         return self.norm(x), new if use_cache else None
+
+    def _forward_train(self, input_ids, cache, use_cache, attention_mask):
+        """``forward`` with the libcyfa embedding and residual norms: each add is
+        taken together with the norm of the branch after it."""
+        x, y = embed_tokens(input_ids, self.embeddings.weight), None
+        new = []
+        for i, layer in enumerate(self.layers):
+            x, h = residual_norm(x, y, layer.attn_norm.weight, eps=layer.attn_norm.eps)
+            y, s = layer.attn(h, None if cache is None else cache[i], use_cache, attention_mask)
+            new.append(s)
+            x, h = residual_norm(x, y, layer.mlp_norm.weight, eps=layer.mlp_norm.eps)
+            y = layer.mlp(h)
+        _, h = residual_norm(x, y, self.norm.weight, eps=self.norm.eps)
+        return h, new if use_cache else None
 
     def _forward_glue(self, input_ids, cache, use_cache, attention_mask):
         """Inference over a sequence (prefill): the blocks of ``forward`` with
@@ -187,6 +216,32 @@ class CyclicFlowAttentionForCausalLM(nn.Module):
 
         save_model(self, directory, tokenizer)
 
+    def fuse_training(self, on=True):
+        """Runs the embedding, the residual norms and the loss of training forwards
+        (bf16 weights on a CUDA device) on the libcyfa operators; returns self."""
+        self.model.fused_training = bool(on)
+        return self
+
+    @torch.no_grad()
+    def score(self, input_ids, attention_mask=None, top=0):
+        """How the model rates a text: for each position t < T - 1 of ``input_ids``
+        [B, T] the log probability of token t + 1 given the tokens up to t, the
+        entropy of that prediction and, for ``top`` > 0, its most likely tokens
+        (``ops.TokenLogProbs`` of [B, T - 1] tensors).  Where ``attention_mask``
+        (right padding) is 0 for the predicted token, logp is 0."""
+        hidden, _ = self.model(input_ids, None, False, attention_mask)
+        targets = input_ids[:, 1:]
+        if attention_mask is not None:
+            targets = targets.masked_fill(attention_mask[:, 1:] == 0, -100)
+        return token_log_probs(self.lm_head(hidden)[:, :-1], targets, top=top)
+
+    def _next_token_loss(self, logits, labels):
+        """Mean cross entropy of labels[:, 1:] (ignoring -100) from logits read in place."""
+        targets = torch.full_like(labels, -100)
+        targets[:, :-1] = labels[:, 1:]
+        logp = token_log_probs(logits, targets).logp
+        return -logp.sum() / (targets != -100).sum()
+
     def _decode_ok(self, input_ids, cache, attention_mask):
         w = self.lm_head.weight
         return (cache is not None and attention_mask is None and input_ids.dim() == 2
@@ -203,7 +258,9 @@ class CyclicFlowAttentionForCausalLM(nn.Module):
         hidden, cache = self.model(input_ids, cache, use_cache, attention_mask)
         logits = self.lm_head(hidden)
         loss = None
-        if labels is not None:
+        if labels is not None and self.model._train_ops_ok(input_ids):
+            loss = self._next_token_loss(logits, labels)
+        elif labels is not None:
             loss = F.cross_entropy(
                 logits[:, :-1].float().reshape(-1, self.config.vocab_size),
                 labels[:, 1:].reshape(-1), ignore_index=-100)

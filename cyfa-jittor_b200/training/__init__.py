@@ -1,3 +1,3 @@
-"""Data-parallel training support: fp32-master AdamW (optim) and resumable
+"""Data-parallel training support: fp32-master AdamW and Muon (optim) and resumable
 training checkpoints (checkpoint), the counterparts of the reference's
 training/optim.py and training/checkpoint.py."""

@@ -1,4 +1,4 @@
-"""AdamW with fp32 master weights and moments, for data-parallel training.
+"""AdamW and Muon with fp32 master weights and moments, for data-parallel training.
 
 Counterpart of the reference's ``training.optim.AdamW`` (training/optim.py:8-124):
 the same constructor, hyperparameter checks, ``backward(loss)`` /
@@ -24,11 +24,14 @@ tensor copies and collectives, so they also run on CPU (gloo) for tests.
 """
 
 import ctypes
+import math
 
 import torch
 import torch.distributed as dist
 
 from cyclic_flow_attention import _lib
+from cyclic_flow_attention.ops import orthogonalize
+from cyclic_flow_attention.ops.orthogonal import QUINTIC
 
 _ALIGN = 8  # elements: 32-byte segment starts for the vectorised kernels
 
@@ -204,21 +207,103 @@ class AdamW:
         _lib.require_cuda(self._master)
         self.update_step += 1
         for group in self.param_groups:
-            lr = group.get("lr", self.lr)
-            b0, b1 = group.get("betas", self.betas)
-            eps = group.get("eps", self.eps)
-            decay = group.get("weight_decay", self.weight_decay)
-            live = [(p, off) for p, off in zip(group["params"], group["offsets"])
-                    if p.requires_grad]
-            if not live:
-                continue
-            arr = (_lib.BucketPiece * len(live))()
-            for i, (p, off) in enumerate(live):
-                if not p.is_contiguous():
-                    raise ValueError("AdamW parameters must be contiguous")
-                arr[i] = _lib.BucketPiece(p.data_ptr(), p.numel(), off, _dtype_code(p))
-            _lib.call("cyfa_adamw_step", arr, len(live), _lib.ptr(self._master),
-                      _lib.ptr(self._m), _lib.ptr(self._v), _lib.ptr(self._grads), float(lr),
-                      float(b0), float(b1), float(eps), float(decay), self.update_step,
-                      _lib.stream())
+            self._update(group)
         self.zero_grad()
+
+    def _live(self, group):
+        """(parameter, offset) pairs of the group's trainable parameters."""
+        live = [(p, off) for p, off in zip(group["params"], group["offsets"]) if p.requires_grad]
+        for p, _ in live:
+            if not p.is_contiguous():
+                raise ValueError("AdamW parameters must be contiguous")
+        return live
+
+    def _update(self, group):
+        lr = group.get("lr", self.lr)
+        b0, b1 = group.get("betas", self.betas)
+        eps = group.get("eps", self.eps)
+        decay = group.get("weight_decay", self.weight_decay)
+        live = self._live(group)
+        if not live:
+            return
+        arr = (_lib.BucketPiece * len(live))()
+        for i, (p, off) in enumerate(live):
+            arr[i] = _lib.BucketPiece(p.data_ptr(), p.numel(), off, _dtype_code(p))
+        _lib.call("cyfa_adamw_step", arr, len(live), _lib.ptr(self._master),
+                  _lib.ptr(self._m), _lib.ptr(self._v), _lib.ptr(self._grads), float(lr),
+                  float(b0), float(b1), float(eps), float(decay), self.update_step,
+                  _lib.stream())
+
+
+def _is_matrix(name, p):
+    return p.dim() == 2 and not any(s in name for s in ("embeddings", "lm_head"))
+
+
+class Muon(AdamW):
+    """Orthogonalised momentum for the matrices, AdamW for everything else.
+
+    A matrix W [rows, cols] with momentum buffer m (the flat ``m`` of AdamW) takes
+
+        m = momentum m + g,   u = g + momentum m  (or m without ``nesterov``)
+        W = W (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) NS(u)
+
+    where NS is ``ops.orthogonalize`` (``steps`` Newton-Schulz steps, the result in
+    bf16); all matrices of one shape go through it in one call.  ``matrix(name,
+    parameter)`` says which parameters these are: by default the two-dimensional
+    ones whose name contains neither "embeddings" nor "lm_head".  The others are
+    updated by AdamW with ``adamw_lr``, ``betas``, ``eps`` and ``adamw_weight_decay``.
+
+    ``params`` is an iterable of tensors or (name, tensor) pairs.  Masters,
+    accumulation, the data-parallel mean, clipping and checkpoints are AdamW's
+    (the matrices' second moments stay zero).
+    """
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.01, steps=5,
+                 coefficients=QUINTIC, matrix=_is_matrix, adamw_lr=1e-4, betas=(0.9, 0.999),
+                 eps=1e-8, adamw_weight_decay=0.01):
+        if lr < 0 or weight_decay < 0 or not 0 <= momentum < 1 or steps < 1:
+            raise ValueError("Invalid Muon hyperparameters")
+        named = [p if isinstance(p, tuple) else (f"0.{i}", p) for i, p in enumerate(params)]
+        matrices = [(n, p) for n, p in named if matrix(n, p)]
+        if any(p.dim() != 2 for _, p in matrices):
+            raise ValueError("Muon's matrices must be two-dimensional")
+        chosen = {id(p) for _, p in matrices}
+        others = [(n, p) for n, p in named if id(p) not in chosen]
+        groups = []
+        if matrices:
+            groups.append({"params": matrices, "matrix": True, "lr": lr,
+                           "weight_decay": weight_decay})
+        if others:
+            groups.append({"params": others})
+        if not groups:
+            raise ValueError("Muon got an empty parameter list")
+        super().__init__(groups, adamw_lr, betas, eps, adamw_weight_decay)
+        self.momentum, self.nesterov = momentum, nesterov
+        self.steps, self.coefficients = steps, tuple(coefficients)
+
+    def _update(self, group):
+        if not group.get("matrix"):
+            return super()._update(group)
+        by_shape = {}
+        for p, off in self._live(group):
+            by_shape.setdefault(tuple(p.shape), []).append((p, off))
+        lr, decay = group["lr"], group["weight_decay"]
+        for (rows, cols), live in by_shape.items():
+            n = len(live)
+            u = torch.empty(n, rows, cols, device=self.device, dtype=torch.float32)
+            if not u.numel():
+                continue
+            arr = (_lib.BucketPiece * n)()
+            for i, (p, off) in enumerate(live):
+                arr[i] = _lib.BucketPiece(u[i].data_ptr(), p.numel(), off, 0)
+            _lib.call("cyfa_muon_momentum", arr, n, _lib.ptr(self._m), _lib.ptr(self._grads),
+                      float(self.momentum), int(self.nesterov), _lib.stream())
+            with torch.no_grad():
+                o = orthogonalize(u, self.steps, self.coefficients)
+            updates = (ctypes.c_void_p * n)()
+            for i, (p, off) in enumerate(live):
+                arr[i] = _lib.BucketPiece(p.data_ptr(), p.numel(), off, _dtype_code(p))
+                updates[i] = o[i].data_ptr()
+            _lib.call("cyfa_muon_apply", arr, updates, n, _lib.ptr(self._master),
+                      float(lr * math.sqrt(max(1.0, rows / cols))), float(1.0 - lr * decay),
+                      _lib.stream())

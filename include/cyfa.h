@@ -560,6 +560,17 @@ int cyfa_adamw_step(const cyfa_bucket_piece* params, int count, float* master, f
                     const float* grad, float lr, float beta1, float beta2, float eps,
                     float weight_decay, int step, void* stream);
 
+/* The element-wise halves of a Muon step (momentum, orthogonalised, applied to the
+ * fp32 master) over the same flat buffers; no counterpart in the reference.
+ * momentum: m = momentum m + grad; u = grad + momentum m (nesterov != 0) or m, written
+ * to each piece's ptr (f32, dtype 0, n elements, 4-byte aligned).
+ * apply: master = master shrink - step_size update, each parameter rounded to its
+ * dtype; updates[i] is parameter i's bf16 update (n elements, 2-byte aligned). */
+int cyfa_muon_momentum(const cyfa_bucket_piece* pieces, int count, float* m, const float* grad,
+                       float momentum, int nesterov, void* stream);
+int cyfa_muon_apply(const cyfa_bucket_piece* params, const void* const* updates, int count,
+                    float* master, float step_size, float shrink, void* stream);
+
 /* Gradient clipping by the global L2 norm.  Replaces: AdamW.clip_grad_norm,
  * training/optim.py:74-89.  grad [n] f32 is scaled in place by
  * min(max_norm / (norm + 1e-6), 1); the norm is written to norm_out (device

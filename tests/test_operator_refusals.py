@@ -131,3 +131,31 @@ def test_c_refusals():
 
     assert ns(work=None) == 2 and ns(Lm=65536) == 1 and ns(m=65537) == 1 and ns(steps=65) == 1
     assert ns(dtype=2) == 4 and ns(nbytes=n - 1) == 7 and ns(work=P(64)) == 3
+
+
+def test_muon_refusals_and_groups():
+    from training.optim import Muon
+
+    w = torch.zeros(4, 6, requires_grad=True)
+    b = torch.zeros(3, requires_grad=True)
+    for kw in (dict(lr=-1.0), dict(momentum=1.0), dict(weight_decay=-0.1), dict(steps=0)):
+        with pytest.raises(ValueError, match="Muon"):
+            Muon([w], **kw)
+    with pytest.raises(ValueError, match="empty"):
+        Muon([])
+    with pytest.raises(ValueError, match="two-dimensional"):
+        Muon([b], matrix=lambda n, p: True)
+    opt = Muon([("x.weight", w), ("lm_head.weight", torch.zeros(4, 6, requires_grad=True)), ("y", b)])
+    assert [g["names"] for g in opt.param_groups] == [["x.weight"], ["lm_head.weight", "y"]]
+    (w.sum() + b.sum()).backward()
+    opt.accumulate_param_grads()
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        opt.step()
+    L = _lib.lib()
+    P = ctypes.c_void_p
+    piece = (_lib.BucketPiece * 1)(_lib.BucketPiece(4096, 8, 0, 0))
+    bad = (_lib.BucketPiece * 1)(_lib.BucketPiece(4096, 8, 4, 0))
+    assert L.cyfa_muon_momentum(None, 1, P(4096), P(4096), 0.9, 1, None) == 2
+    assert L.cyfa_muon_momentum(bad, 1, P(4096), P(4096), 0.9, 1, None) == 3
+    assert L.cyfa_muon_momentum(piece, -1, P(4096), P(4096), 0.9, 1, None) == 1
+    assert L.cyfa_muon_apply(piece, None, 1, P(4096), 0.1, 1.0, None) == 2
