@@ -9,9 +9,9 @@
 // that keeps the lo parts of small entries above fp16's underflow and leaves room
 // up to |entry| < 16.  A product is the three MMAs hi hi + hi lo + lo hi where its
 // rounding would show, one MMA hi hi where it does not: a X + B X cancels to a
-// tenth of its terms once the singular values are near 1, so in the last three
-// steps A A and B X take all three; A = X X^T (whose error is not cancelled
-// against anything) and every product of the earlier steps take one.  Simulated
+// tenth of its terms once the singular values are near 1, so A A and B X take all
+// three except in the first two steps (while most of them are small); A = X X^T,
+// whose error is not cancelled against anything, takes one.  Simulated
 // in 64 bits on Gaussian, low-rank and graded matrices this is within 1.5e-4 to
 // 6e-4 relative of the exact iteration, a third of the bf16 rounding of the
 // result (1.7e-3); one MMA everywhere is up to 2.8e-3 off, three everywhere 8e-7,
@@ -33,8 +33,13 @@ template <int PROD>
 constexpr int ns_threads() {
   return (ns_epi_warps<PROD>() + 2) * 32;
 }
-constexpr int kNsFullSteps = 3;  // last steps with three-MMA products
+// Steps whose A A and B X take three MMAs: all but the first two, and the last three.
+__host__ __device__ constexpr bool ns_full_step(int step, int steps) {
+  return step >= 2 || steps - step <= 3;
+}
 constexpr int kNsTile = 256;  // rows and columns of a CTA pair's tile
+constexpr long long kNsTinyEntries = 16384;  // below: rounding errors average over too few
+constexpr int kNsSmallTiles = 4;  // column tiles of a matrix that one pair works through
 
 enum NsMode : int {
   kNsGram = 0,    // D = acc
@@ -50,6 +55,7 @@ struct NsGemmParams {
   float alpha, beta;
   __nv_bfloat16* out;       // kNsLast
   int tall;                 // out is [L, cols, M]
+  int one;                  // PROD 4: one MMA a product
 };
 
 // Per stage and CTA: 128 rows of A and 128 of B, 64 contraction columns each, hi
@@ -58,11 +64,11 @@ constexpr int kNsPart = 128 * 128;
 constexpr int kNsSlot = 32 * 64;  // a finishing warp's block: 32 rows x 32 columns of 16 bits
 template <int PROD>
 constexpr int ns_stage_bytes() {
-  return (PROD == 3 ? 4 : 2) * kNsPart;
+  return (PROD >= 3 ? 4 : 2) * kNsPart;
 }
 template <int PROD>
 constexpr int ns_stages() {
-  return PROD == 3 ? 3 : 5;
+  return PROD == 4 ? 2 : (PROD == 3 ? 3 : 5);
 }
 template <int PROD>
 constexpr int ns_smem() {
@@ -230,83 +236,70 @@ struct NsEpiMaps {
 // loads (one lane), one of the leader's issues the MMAs of both CTAs (one lane), the
 // EPI others finish the tile from one of the two TMEM accumulators while the next
 // tile is computed into the other: warp w reads lane quadrant w & 3 (32 rows) and
-// the columns (1024 / EPI) (w >> 2) .., 32 at a time.  PROD: MMAs per product (3: hi and lo parts).
+// the columns (1024 / EPI) (w >> 2) .., 32 at a time.  PROD: MMAs per
+// product (3: hi and lo parts; 4: one or three as p.one says, in the shape for small
+// matrices: fewer columns a tile and more finishing warps, for latency).
+template <int PROD>
+struct NsBarriers {
+  uint64_t full[ns_stages<PROD>()], empty[ns_stages<PROD>()], t_full[2], t_empty[2];
+  uint64_t c_full[ns_epi_warps<PROD>()];
+};
+// What a thread carries from one product to the next.
+template <int PROD>
+struct NsCta {
+  NsBarriers<PROD>* b;
+  uint8_t* smem;
+  volatile int* abort_flag;
+  uint32_t tmem;
+  int rank;
+  int q = 0, i = 0;  // ring uses (finishing warps: C blocks) and tiles so far
+};
+struct NsMaps {
+  const CUtensorMap *ah, *al, *bh, *bl, *ch, *cl, *dh, *dl;
+};
+
+// The tiles first, first + step, .. < end of one product.
 template <int PROD, int MODE>
-__global__ void __launch_bounds__(ns_threads<PROD>(), 1)
-    ns_gemm_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_constant__ CUtensorMap map_al,
-                   const __grid_constant__ CUtensorMap map_bh, const __grid_constant__ CUtensorMap map_bl,
-                   const __grid_constant__ NsEpiMaps em, NsGemmParams p) {
+__device__ __forceinline__ void ns_product(NsCta<PROD>& cta, const NsMaps& mp, const NsGemmParams& p,
+                                           int first, int step, int end) {
   constexpr bool SYM = MODE == kNsGram || MODE == kNsPoly;
   constexpr int kStage = ns_stage_bytes<PROD>(), kStages = ns_stages<PROD>();
   constexpr int kEpi = ns_epi_warps<PROD>();
   constexpr int kB = kStage / 2;  // B parts follow the A parts
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~uintptr_t(1023));
-  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], t_full[2], t_empty[2];
-  __shared__ __align__(8) uint64_t c_full[kEpi];
-  __shared__ uint32_t tmem_base;
-  __shared__ int s_abort;
-  volatile int* abort_flag = &s_abort;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rank = int(cluster_rank()), pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
-  if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&t_full[i], 1);
-      mbar_init(&t_empty[i], 2 * kEpi);
-    }
-    for (int i = 0; i < kEpi; ++i) mbar_init(&c_full[i], 1);
-    s_abort = 0;
-    mbar_fence_init();
-    prefetch_tmap(&map_ah);
-    prefetch_tmap(&map_bh);
-  }
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_u32(&tmem_base)),
-                 "r"(2 * kNsTile));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
-  }
-  tc_fence_before();
-  __syncthreads();
-  cluster_sync_all();  // the peer's barriers are ready
-  tc_fence_after();
-  pdl_wait();
-  pdl_trigger();
-  const uint32_t tmem = tmem_base;
+  uint8_t* const smem = cta.smem;
+  volatile int* const abort_flag = cta.abort_flag;
+  const uint32_t tmem = cta.tmem;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = cta.rank;
   const int nk = (p.K + 63) / 64;
-
+  const bool lo = PROD == 3 || (PROD == 4 && !p.one);             // three MMAs
+  const int tn = PROD == 4 && p.cols <= 128 ? 128 : kNsTile;       // columns of a tile
   if (warp == kEpi) {
     if (lane == 0) {
-      int q = 0;
+      int& q = cta.q;
       bool ok = true;
-      for (int u = pair; ok && u < p.nunits && !*abort_flag; u += npairs) {
+      for (int u = first; ok && u < end && !*abort_flag; u += step) {
         const NsTile t = ns_tile<SYM>(p, u);
-        const int ra = t.ti * kNsTile + rank * 128, cb = t.tj * kNsTile + rank * 128;
+        const int ra = t.ti * kNsTile + rank * 128, cb = t.tj * kNsTile + rank * (tn / 2);
         for (int k = 0; k < nk; ++k, ++q) {
           const int s = q % kStages;
-          if (q >= kStages && !mbar_wait(&empty[s], ((q / kStages) - 1) & 1)) {
+          if (q >= kStages && !mbar_wait(&cta.b->empty[s], ((q / kStages) - 1) & 1)) {
             ok = false;
             break;
           }
           uint8_t* st = smem + s * kStage;
-          const uint32_t bar = cluster_map(smem_u32(&full[s]), 0);
-          if (rank == 0) mbar_expect_tx(&full[s], 2 * kStage);  // both CTAs' bytes
-          pair_load_3d(st, &map_ah, bar, 64 * k, ra, t.l);
-          if (PROD == 3) pair_load_3d(st + kNsPart, &map_al, bar, 64 * k, ra, t.l);
+          const uint32_t bar = cluster_map(smem_u32(&cta.b->full[s]), 0);
+          if (rank == 0) mbar_expect_tx(&cta.b->full[s], PROD == 1 || lo ? 2 * kStage : kStage);  // both CTAs' bytes
+          pair_load_3d(st, mp.ah, bar, 64 * k, ra, t.l);
+          if (lo) pair_load_3d(st + kNsPart, mp.al, bar, 64 * k, ra, t.l);
           if (SYM) {
-            pair_load_3d(st + kB, &map_bh, bar, 64 * k, cb, t.l);
-            if (PROD == 3) pair_load_3d(st + kB + kNsPart, &map_bl, bar, 64 * k, cb, t.l);
+            pair_load_3d(st + kB, mp.bh, bar, 64 * k, cb, t.l);
+            if (lo) pair_load_3d(st + kB + kNsPart, mp.bl, bar, 64 * k, cb, t.l);
           } else {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              pair_load_3d(st + kB + c * 8192, &map_bh, bar, cb + 64 * c, 64 * k, t.l);
-              if (PROD == 3)
-                pair_load_3d(st + kB + kNsPart + c * 8192, &map_bl, bar, cb + 64 * c, 64 * k, t.l);
+              pair_load_3d(st + kB + c * 8192, mp.bh, bar, cb + 64 * c, 64 * k, t.l);
+              if (lo)
+                pair_load_3d(st + kB + kNsPart + c * 8192, mp.bl, bar, cb + 64 * c, 64 * k, t.l);
             }
           }
         }
@@ -316,18 +309,18 @@ __global__ void __launch_bounds__(ns_threads<PROD>(), 1)
       // CTAs' copies, the peer stays until the cluster barrier below
       if (rank == 0)
         for (int j = q > kStages ? q - kStages : 0; j < q; ++j)
-          mbar_wait(&full[j % kStages], (j / kStages) & 1);
+          mbar_wait(&cta.b->full[j % kStages], (j / kStages) & 1);
     }
   } else if (warp == kEpi + 1) {
     if (lane == 0 && rank == 0) {
-      const uint32_t idesc = ns_idesc(kNsTile, kNsTile, SYM ? 0 : 1);
-      int q = 0, i = 0;
+      const uint32_t idesc = ns_idesc(kNsTile, tn, SYM ? 0 : 1);
+      int &q = cta.q, &i = cta.i;
       uint64_t* last_bar = nullptr;
       uint32_t last_par = 0;
       bool ok = true;
-      for (int u = pair; ok && u < p.nunits && !*abort_flag; u += npairs, ++i) {
+      for (int u = first; ok && u < end && !*abort_flag; u += step, ++i) {
         const int b = i & 1;
-        if (i >= 2 && !mbar_wait(&t_empty[b], ((i >> 1) - 1) & 1)) {
+        if (i >= 2 && !mbar_wait(&cta.b->t_empty[b], ((i >> 1) - 1) & 1)) {
           ok = false;
           break;
         }
@@ -335,7 +328,7 @@ __global__ void __launch_bounds__(ns_threads<PROD>(), 1)
         const uint32_t acc = tmem + b * kNsTile;
         for (int k = 0; k < nk; ++k, ++q) {
           const int s = q % kStages;
-          if (!mbar_wait(&full[s], (q / kStages) & 1)) {
+          if (!mbar_wait(&cta.b->full[s], (q / kStages) & 1)) {
             ok = false;
             break;
           }
@@ -345,7 +338,7 @@ __global__ void __launch_bounds__(ns_threads<PROD>(), 1)
           for (int ks = 0; ks < 4; ++ks) {
             const uint64_t dah = kmaj_desc(ah, 128, ks);
             const uint64_t dbh = SYM ? kmaj_desc(bh, 128, ks) : mnmaj_desc(bh, 64, ks);
-            if (PROD == 3) {
+            if (lo) {
               const uint64_t dal = kmaj_desc(ah + kNsPart, 128, ks);
               const uint64_t dbl = SYM ? kmaj_desc(bh + kNsPart, 128, ks)
                                        : mnmaj_desc(bh + kNsPart, 64, ks);
@@ -356,20 +349,20 @@ __global__ void __launch_bounds__(ns_threads<PROD>(), 1)
               pair_umma(acc, dah, dbh, idesc, k > 0 || ks > 0);
             }
           }
-          pair_commit(&empty[s]);
-          last_bar = &empty[s];
+          pair_commit(&cta.b->empty[s]);
+          last_bar = &cta.b->empty[s];
           last_par = (q / kStages) & 1;
         }
         if (!ok) break;
-        pair_commit(&t_full[b]);
-        last_bar = &t_full[b];
+        pair_commit(&cta.b->t_full[b]);
+        last_bar = &cta.b->t_full[b];
         last_par = (i >> 1) & 1;
       }
       if (!ok) *abort_flag = 1;
       if (last_bar) mbar_wait(last_bar, last_par);  // all issued MMAs are done
     }
   } else {
-    constexpr int kCols = 1024 / kEpi;  // of this warp
+    const int kCols = tn * 4 / kEpi;  // of this warp
     const int quad = warp & 3, group = warp >> 2;
     uint8_t* slot = smem + kStages * kStage + warp * 2 * kNsSlot;
     const uint32_t bh = smem_u32(slot), bl = bh + kNsSlot;  // hi and lo block
@@ -377,17 +370,17 @@ __global__ void __launch_bounds__(ns_threads<PROD>(), 1)
     constexpr float kDown = 1.f / kNsScale;
     const float al = (MODE == kNsPoly ? p.alpha : 1.f) * kDown;
     bool stores = false;  // bulk stores issued (lane 0)
-    int cq = 0;           // C blocks so far
+    int& cq = cta.q;        // C blocks so far
+    int& i = cta.i;
     auto fetch_c = [&](int c, int r, int l) {
       if (lane == 0) {
         if (stores) bulk_wait_read_all();  // the blocks' last contents have left
-        mbar_expect_tx(&c_full[warp], 2 * kNsSlot);
-        tma_load_3d(slot, &em.ch, &c_full[warp], c, r, l);
-        tma_load_3d(slot + kNsSlot, &em.cl, &c_full[warp], c, r, l);
+        mbar_expect_tx(&cta.b->c_full[warp], 2 * kNsSlot);
+        tma_load_3d(slot, mp.ch, &cta.b->c_full[warp], c, r, l);
+        tma_load_3d(slot + kNsSlot, mp.cl, &cta.b->c_full[warp], c, r, l);
       }
     };
-    int i = 0;
-    for (int u = pair; u < p.nunits; u += npairs, ++i) {
+    for (int u = first; u < end; u += step, ++i) {
       const int b = i & 1;
       const NsTile t = ns_tile<SYM>(p, u);
       const int r0 = t.ti * kNsTile + rank * 128 + quad * 32;
@@ -398,10 +391,10 @@ __global__ void __launch_bounds__(ns_threads<PROD>(), 1)
       // they finish
       if (HAS_C && work) fetch_c(col0, r0, t.l);
       const bool got =
-          __all_sync(0xffffffffu, *abort_flag == 0 && mbar_wait(&t_full[b], (i >> 1) & 1));
+          __all_sync(0xffffffffu, *abort_flag == 0 && mbar_wait(&cta.b->t_full[b], (i >> 1) & 1));
       if (!got) {
         *abort_flag = 1;
-        if (HAS_C && work) mbar_wait(&c_full[warp], cq & 1);  // the copies land first
+        if (HAS_C && work) mbar_wait(&cta.b->c_full[warp], cq & 1);  // the copies land first
         break;
       }
       tc_fence_after();
@@ -414,7 +407,7 @@ __global__ void __launch_bounds__(ns_threads<PROD>(), 1)
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] *= al;
         if (HAS_C) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&c_full[warp], cq & 1))) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&cta.b->c_full[warp], cq & 1))) {
             *abort_flag = 1;
             break;
           }
@@ -453,8 +446,8 @@ __global__ void __launch_bounds__(ns_threads<PROD>(), 1)
           fence_async_smem();
           __syncwarp();
           if (lane == 0) {
-            tma_store_3d(&em.dh, slot, c0, r0, t.l);
-            tma_store_3d(&em.dl, slot + kNsSlot, c0, r0, t.l);
+            tma_store_3d(mp.dh, slot, c0, r0, t.l);
+            tma_store_3d(mp.dl, slot + kNsSlot, c0, r0, t.l);
             bulk_commit();
             stores = true;
           }
@@ -470,8 +463,8 @@ __global__ void __launch_bounds__(ns_threads<PROD>(), 1)
             fence_async_smem();
             __syncwarp();
             if (lane == 0) {
-              tma_store_3d(&em.dh, slot, r0, c0, t.l);
-              tma_store_3d(&em.dl, slot + kNsSlot, r0, c0, t.l);
+              tma_store_3d(mp.dh, slot, r0, c0, t.l);
+              tma_store_3d(mp.dl, slot + kNsSlot, r0, c0, t.l);
               bulk_commit();
             }
           }
@@ -480,18 +473,143 @@ __global__ void __launch_bounds__(ns_threads<PROD>(), 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) cluster_arrive(cluster_map(smem_u32(&t_empty[b]), 0));
+      if (lane == 0) cluster_arrive(cluster_map(smem_u32(&cta.b->t_empty[b]), 0));
     }
     if (lane == 0 && stores) bulk_wait_all();
   }
+}
+
+// Shared memory, barriers and TMEM of a CTA of a pair; all threads of both CTAs.
+template <int PROD>
+__device__ __forceinline__ NsCta<PROD> ns_open(uint8_t* smem_raw, NsBarriers<PROD>* b, uint32_t* tmem_base,
+                                               int* abort_flag) {
+  constexpr int kStages = ns_stages<PROD>(), kEpi = ns_epi_warps<PROD>();
+  const int tid = threadIdx.x;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&b->full[i], 1);
+      mbar_init(&b->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&b->t_full[i], 1);
+      mbar_init(&b->t_empty[i], 2 * kEpi);
+    }
+    for (int i = 0; i < kEpi; ++i) mbar_init(&b->c_full[i], 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (tid < 32) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_base)),
+                 "r"(2 * kNsTile));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the peer's barriers are ready
+  tc_fence_after();
+  NsCta<PROD> c;
+  c.b = b;
+  c.smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  c.abort_flag = abort_flag;
+  c.tmem = *tmem_base;
+  c.rank = int(cluster_rank());
+  return c;
+}
+__device__ __forceinline__ void ns_close(uint32_t tmem) {
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // neither CTA leaves while the other may signal or read it
-  if (warp == 0) {
+  if (threadIdx.x < 32) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"(2 * kNsTile));
   }
+}
+
+template <int PROD, int MODE>
+__global__ void __launch_bounds__(ns_threads<PROD>(), 1)
+    ns_gemm_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_constant__ CUtensorMap map_al,
+                   const __grid_constant__ CUtensorMap map_bh, const __grid_constant__ CUtensorMap map_bl,
+                   const __grid_constant__ NsEpiMaps em, NsGemmParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) NsBarriers<PROD> bars;
+  __shared__ uint32_t tmem_base;
+  __shared__ int s_abort;
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&map_ah);
+    prefetch_tmap(&map_bh);
+  }
+  NsCta<PROD> c = ns_open<PROD>(smem_raw, &bars, &tmem_base, &s_abort);
+  pdl_wait();
+  pdl_trigger();
+  const NsMaps m{&map_ah, &map_al, &map_bh, &map_bl, &em.ch, &em.cl, &em.dh, &em.dl};
+  ns_product<PROD, MODE>(c, m, p, blockIdx.x >> 1, gridDim.x >> 1, p.nunits);
+  ns_close(c.tmem);
+}
+
+// Matrices of one tile row (M <= 256): every product of a matrix belongs to one CTA
+// pair, which runs all steps of its matrices in one launch.  The pair's barrier and
+// proxy fences stand between a product's stores and the next one's loads.
+struct NsAllMaps {  // [part: hi, lo], X twice
+  CUtensorMap xa[2][2], xk[2][2], xe[2][2], aa[2], ae[2], ba[2], be[2];
+};
+__device__ __forceinline__ void ns_between() {
+  // the storing threads have waited for their copies; the barrier's release and
+  // acquire order them before the peer's work, the fences across the proxies
+  asm volatile("fence.proxy.async;" ::: "memory");
+  __syncwarp();
+  cluster_sync_all();
+  asm volatile("fence.proxy.async;" ::: "memory");
+}
+
+__global__ void __launch_bounds__(ns_threads<4>(), 1)
+    ns_small_kernel(const __grid_constant__ NsAllMaps w, NsGemmParams p, int N, int steps, float a,
+                    float b, float c2) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) NsBarriers<4> bars;
+  __shared__ uint32_t tmem_base;
+  __shared__ int s_abort;
+  if (threadIdx.x < int(sizeof(NsAllMaps) / sizeof(CUtensorMap)))
+    prefetch_tmap(reinterpret_cast<const CUtensorMap*>(&w) + threadIdx.x);
+  NsCta<4> c = ns_open<4>(smem_raw, &bars, &tmem_base, &s_abort);
+  pdl_wait();
+  pdl_trigger();
+  const int tiles = (N + kNsTile - 1) / kNsTile;
+  p.tiles_m = 1;
+  for (int l = blockIdx.x >> 1; l < p.L; l += gridDim.x >> 1) {
+    for (int step = 0; step < steps; ++step) {
+      const int i = step & 1, last = step == steps - 1;
+      const bool all = (long long)p.M * N < kNsTinyEntries, full = all || ns_full_step(step, steps);
+      p.per = 1;
+      p.cols = p.M;
+      p.K = N;
+      p.one = !all;
+      const NsMaps gram{&w.xa[i][0], &w.xa[i][1], &w.xa[i][0], &w.xa[i][1],
+                        nullptr,     nullptr,     &w.ae[0],    &w.ae[1]};
+      ns_product<4, kNsGram>(c, gram, p, l, 1, l + 1);
+      ns_between();
+      p.K = p.M;
+      p.one = !full;
+      p.alpha = c2;
+      p.beta = b;
+      const NsMaps poly{&w.aa[0], &w.aa[1], &w.aa[0], &w.aa[1],
+                        &w.ae[0], &w.ae[1], &w.be[0], &w.be[1]};
+      ns_product<4, kNsPoly>(c, poly, p, l, 1, l + 1);
+      ns_between();
+      p.per = tiles;
+      p.cols = N;
+      p.beta = a;
+      const NsMaps next{&w.ba[0],    &w.ba[1],    &w.xk[i][0],     &w.xk[i][1],
+                        &w.xe[i][0], &w.xe[i][1], &w.xe[1 - i][0], &w.xe[1 - i][1]};
+      if (last)
+        ns_product<4, kNsLast>(c, next, p, l * tiles, 1, (l + 1) * tiles);
+      else
+        ns_product<4, kNsStep>(c, next, p, l * tiles, 1, (l + 1) * tiles);
+      ns_between();
+    }
+  }
+  ns_close(c.tmem);
 }
 
 // Partial sums of squares: 8 entries at a time in fp32, the sums of those in 64
@@ -768,53 +886,58 @@ int cyfa_newton_schulz(const void* g, int dtype, int L, int m, int n, int steps,
   // rows x 64 columns of X, A and B for the operands read along their rows, 64 x 64
   // of X for B X, where X is read down its columns
   // and 32 x 32 blocks for the finishing warps
-  CUtensorMap xa[2][2], xk[2][2], xe[2][2], aa[2], ba[2], ae[2], be[2];
+  NsAllMaps t;
   for (int h = 0; h < 2; ++h) {
     int rc = kOk;
     for (int i = 0; i < 2 && !rc; ++i) {
       const __half* x = h ? w.xl[i] : w.xh[i];
-      rc = ns_tmap(&xa[i][h], x, L, w.M, w.N, w.ldx, 64, 128);
-      if (!rc) rc = ns_tmap(&xk[i][h], x, L, w.M, w.N, w.ldx, 64, 64);
-      if (!rc) rc = ns_tmap(&xe[i][h], x, L, w.M, w.N, w.ldx, 32, 32);
+      rc = ns_tmap(&t.xa[i][h], x, L, w.M, w.N, w.ldx, 64, 128);
+      if (!rc) rc = ns_tmap(&t.xk[i][h], x, L, w.M, w.N, w.ldx, 64, 64);
+      if (!rc) rc = ns_tmap(&t.xe[i][h], x, L, w.M, w.N, w.ldx, 32, 32);
     }
     const __half *a_ = h ? w.al : w.ah, *b_ = h ? w.bl : w.bh;
-    if (!rc) rc = ns_tmap(&aa[h], a_, L, w.M, w.M, w.lda, 64, 128);
-    if (!rc) rc = ns_tmap(&ae[h], a_, L, w.M, w.M, w.lda, 32, 32);
-    if (!rc) rc = ns_tmap(&ba[h], b_, L, w.M, w.M, w.lda, 64, 128);
-    if (!rc) rc = ns_tmap(&be[h], b_, L, w.M, w.M, w.lda, 32, 32);
+    if (!rc) rc = ns_tmap(&t.aa[h], a_, L, w.M, w.M, w.lda, 64, 128);
+    if (!rc) rc = ns_tmap(&t.ae[h], a_, L, w.M, w.M, w.lda, 32, 32);
+    if (!rc) rc = ns_tmap(&t.ba[h], b_, L, w.M, w.M, w.lda, 64, 128);
+    if (!rc) rc = ns_tmap(&t.be[h], b_, L, w.M, w.M, w.lda, 32, 32);
     if (rc) return rc;
+  }
+  NsGemmParams q{};
+  q.L = L;
+  q.M = w.M;
+  q.out = o;
+  q.tall = tall;
+  // matrices of one tile row and a few columns' tiles: one launch for all steps
+  const int tiles_n = (w.N + kNsTile - 1) / kNsTile;
+  if (w.M <= kNsTile && (tiles_n <= kNsSmallTiles || L >= 74)) {
+    set_smem(ns_small_kernel, ns_smem<4>());
+    CYFA_LAUNCH("ns_small", s,
+                (launch_cluster_k(ns_small_kernel, 2 * unsigned(std::min(L, 74)), ns_threads<4>(), 2,
+                                  ns_smem<4>(), s, t, q, w.N, steps, a, b, c)));
+    return launch_status();
   }
   for (int step = 0; step < steps; ++step) {
     const int i = step & 1, last = step == steps - 1;
-    // matrices of one tile row: rounding errors average over few entries, and the
-    // time is the launches' latency
-    const bool all = w.M <= kNsTile, full = all || steps - step <= kNsFullSteps;
-    NsGemmParams p{};
-    p.L = L;
-    p.M = w.M;
-    p.out = o;
-    p.tall = tall;
+    const bool full = ns_full_step(step, steps);
+    NsGemmParams p = q;
     p.cols = w.M;
     p.K = w.N;
-    if (all)
-      CYFA_LAUNCH("ns_gram", s, (ns_launch<3, kNsGram>(xa[i], xa[i], ae, ae, p, s)));
-    else
-      CYFA_LAUNCH("ns_gram_1", s, (ns_launch<1, kNsGram>(xa[i], xa[i], ae, ae, p, s)));
+    CYFA_LAUNCH("ns_gram_1", s, (ns_launch<1, kNsGram>(t.xa[i], t.xa[i], t.ae, t.ae, p, s)));
     p.K = w.M;
     p.alpha = c;
     p.beta = b;
     if (full)
-      CYFA_LAUNCH("ns_poly", s, (ns_launch<3, kNsPoly>(aa, aa, ae, be, p, s)));
+      CYFA_LAUNCH("ns_poly", s, (ns_launch<3, kNsPoly>(t.aa, t.aa, t.ae, t.be, p, s)));
     else
-      CYFA_LAUNCH("ns_poly_1", s, (ns_launch<1, kNsPoly>(aa, aa, ae, be, p, s)));
+      CYFA_LAUNCH("ns_poly_1", s, (ns_launch<1, kNsPoly>(t.aa, t.aa, t.ae, t.be, p, s)));
     p.cols = w.N;
     p.beta = a;
     if (last)
-      CYFA_LAUNCH("ns_last", s, (ns_launch<3, kNsLast>(ba, xk[i], xe[i], xe[i], p, s)));
+      CYFA_LAUNCH("ns_last", s, (ns_launch<3, kNsLast>(t.ba, t.xk[i], t.xe[i], t.xe[i], p, s)));
     else if (full)
-      CYFA_LAUNCH("ns_step", s, (ns_launch<3, kNsStep>(ba, xk[i], xe[i], xe[1 - i], p, s)));
+      CYFA_LAUNCH("ns_step", s, (ns_launch<3, kNsStep>(t.ba, t.xk[i], t.xe[i], t.xe[1 - i], p, s)));
     else
-      CYFA_LAUNCH("ns_step_1", s, (ns_launch<1, kNsStep>(ba, xk[i], xe[i], xe[1 - i], p, s)));
+      CYFA_LAUNCH("ns_step_1", s, (ns_launch<1, kNsStep>(t.ba, t.xk[i], t.xe[i], t.xe[1 - i], p, s)));
   }
   return launch_status();
 }
