@@ -38,8 +38,11 @@ __host__ __device__ constexpr bool ns_full_step(int step, int steps) {
   return step >= 2 || steps - step <= 3;
 }
 constexpr int kNsTile = 256;  // rows and columns of a CTA pair's tile
-constexpr long long kNsTinyEntries = 16384;  // below: rounding errors average over too few
-constexpr int kNsSmallTiles = 4;  // column tiles of a matrix that one pair works through
+// Matrices whose rounding errors average over too few entries to be left at one MMA.
+__host__ __device__ constexpr bool ns_tiny(int M, int N) {
+  return M < 32 || (long long)M * N < 16384;
+}
+constexpr int kNsSoloWidth = 2048;  // columns of a matrix that one CTA works through
 
 enum NsMode : int {
   kNsGram = 0,    // D = acc
@@ -55,7 +58,8 @@ struct NsGemmParams {
   float alpha, beta;
   __nv_bfloat16* out;       // kNsLast
   int tall;                 // out is [L, cols, M]
-  int one;                  // PROD 4: one MMA a product
+  int one;                  // small matrices: one MMA a product
+  float diag;               // and a in the units of D, added to B's diagonal
 };
 
 // Per stage and CTA: 128 rows of A and 128 of B, 64 contraction columns each, hi
@@ -64,11 +68,11 @@ constexpr int kNsPart = 128 * 128;
 constexpr int kNsSlot = 32 * 64;  // a finishing warp's block: 32 rows x 32 columns of 16 bits
 template <int PROD>
 constexpr int ns_stage_bytes() {
-  return (PROD >= 3 ? 4 : 2) * kNsPart;
+  return (PROD == 3 ? 4 : 2) * kNsPart;
 }
 template <int PROD>
 constexpr int ns_stages() {
-  return PROD == 4 ? 2 : (PROD == 3 ? 3 : 5);
+  return PROD == 3 ? 3 : 5;
 }
 template <int PROD>
 constexpr int ns_smem() {
@@ -206,21 +210,47 @@ __device__ __forceinline__ void pair_load_3d(void* dst, const void* tmap, uint32
       "l"(tmap), "r"(bar), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
-__device__ __forceinline__ void pair_umma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
-                                          uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+// The MMA warp runs converged, all its addresses warp-uniform, and one lane issues:
+// with a single lane inside a divergent branch each operand was moved to the uniform
+// registers for every instruction, 1400 cycles for a 64-column block whose MMAs take
+// 512 (one) or 1536 (three).
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t e;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
+  return e;
 }
-// Arrives on the barrier at this address in both CTAs when the MMAs issued so far
-// are done.
-__device__ __forceinline__ void pair_commit(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
-      " [%0], %1;" ::"r"(smem_u32(bar)),
-      "h"(static_cast<uint16_t>(3))
-      : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void ns_umma(uint32_t lane_on, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                        uint32_t idesc, uint32_t accumulate) {
+  if (PAIR)
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lane_on));
+  else
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lane_on));
+}
+// Arrives on the barrier (PAIR: at this address in both CTAs) when the MMAs issued so
+// far are done.
+template <bool PAIR>
+__device__ __forceinline__ void ns_commit(uint32_t lane_on, uint64_t* bar) {
+  if (PAIR)
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
+        " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;\n}\n" ::"r"(smem_u32(bar)),
+        "h"(static_cast<uint16_t>(3)), "r"(lane_on)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(
+            smem_u32(bar)),
+        "r"(lane_on)
+        : "memory");
 }
 __device__ __forceinline__ void cluster_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -237,8 +267,7 @@ struct NsEpiMaps {
 // EPI others finish the tile from one of the two TMEM accumulators while the next
 // tile is computed into the other: warp w reads lane quadrant w & 3 (32 rows) and
 // the columns (1024 / EPI) (w >> 2) .., 32 at a time.  PROD: MMAs per
-// product (3: hi and lo parts; 4: one or three as p.one says, in the shape for small
-// matrices: fewer columns a tile and more finishing warps, for latency).
+// product (3: hi and lo parts).
 template <int PROD>
 struct NsBarriers {
   uint64_t full[ns_stages<PROD>()], empty[ns_stages<PROD>()], t_full[2], t_empty[2];
@@ -269,17 +298,16 @@ __device__ __forceinline__ void ns_product(NsCta<PROD>& cta, const NsMaps& mp, c
   uint8_t* const smem = cta.smem;
   volatile int* const abort_flag = cta.abort_flag;
   const uint32_t tmem = cta.tmem;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = cta.rank;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, rank = cta.rank;
   const int nk = (p.K + 63) / 64;
-  const bool lo = PROD == 3 || (PROD == 4 && !p.one);             // three MMAs
-  const int tn = PROD == 4 && p.cols <= 128 ? 128 : kNsTile;       // columns of a tile
+  constexpr bool lo = PROD == 3;
   if (warp == kEpi) {
     if (lane == 0) {
       int& q = cta.q;
       bool ok = true;
       for (int u = first; ok && u < end && !*abort_flag; u += step) {
         const NsTile t = ns_tile<SYM>(p, u);
-        const int ra = t.ti * kNsTile + rank * 128, cb = t.tj * kNsTile + rank * (tn / 2);
+        const int ra = t.ti * kNsTile + rank * 128, cb = t.tj * kNsTile + rank * 128;
         for (int k = 0; k < nk; ++k, ++q) {
           const int s = q % kStages;
           if (q >= kStages && !mbar_wait(&cta.b->empty[s], ((q / kStages) - 1) & 1)) {
@@ -288,7 +316,7 @@ __device__ __forceinline__ void ns_product(NsCta<PROD>& cta, const NsMaps& mp, c
           }
           uint8_t* st = smem + s * kStage;
           const uint32_t bar = cluster_map(smem_u32(&cta.b->full[s]), 0);
-          if (rank == 0) mbar_expect_tx(&cta.b->full[s], PROD == 1 || lo ? 2 * kStage : kStage);  // both CTAs' bytes
+          if (rank == 0) mbar_expect_tx(&cta.b->full[s], 2 * kStage);  // both CTAs' bytes
           pair_load_3d(st, mp.ah, bar, 64 * k, ra, t.l);
           if (lo) pair_load_3d(st + kNsPart, mp.al, bar, 64 * k, ra, t.l);
           if (SYM) {
@@ -312,15 +340,16 @@ __device__ __forceinline__ void ns_product(NsCta<PROD>& cta, const NsMaps& mp, c
           mbar_wait(&cta.b->full[j % kStages], (j / kStages) & 1);
     }
   } else if (warp == kEpi + 1) {
-    if (lane == 0 && rank == 0) {
-      const uint32_t idesc = ns_idesc(kNsTile, tn, SYM ? 0 : 1);
+    if (rank == 0) {
+      const uint32_t on = elect_lane();
+      const uint32_t idesc = ns_idesc(kNsTile, kNsTile, SYM ? 0 : 1);
       int &q = cta.q, &i = cta.i;
       uint64_t* last_bar = nullptr;
       uint32_t last_par = 0;
       bool ok = true;
-      for (int u = first; ok && u < end && !*abort_flag; u += step, ++i) {
+      for (int u = first; ok && u < end && !__any_sync(0xffffffffu, *abort_flag); u += step, ++i) {
         const int b = i & 1;
-        if (i >= 2 && !mbar_wait(&cta.b->t_empty[b], ((i >> 1) - 1) & 1)) {
+        if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(&cta.b->t_empty[b], ((i >> 1) - 1) & 1))) {
           ok = false;
           break;
         }
@@ -328,7 +357,7 @@ __device__ __forceinline__ void ns_product(NsCta<PROD>& cta, const NsMaps& mp, c
         const uint32_t acc = tmem + b * kNsTile;
         for (int k = 0; k < nk; ++k, ++q) {
           const int s = q % kStages;
-          if (!mbar_wait(&cta.b->full[s], (q / kStages) & 1)) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&cta.b->full[s], (q / kStages) & 1))) {
             ok = false;
             break;
           }
@@ -342,19 +371,19 @@ __device__ __forceinline__ void ns_product(NsCta<PROD>& cta, const NsMaps& mp, c
               const uint64_t dal = kmaj_desc(ah + kNsPart, 128, ks);
               const uint64_t dbl = SYM ? kmaj_desc(bh + kNsPart, 128, ks)
                                        : mnmaj_desc(bh + kNsPart, 64, ks);
-              pair_umma(acc, dal, dbh, idesc, k > 0 || ks > 0);
-              pair_umma(acc, dah, dbl, idesc, 1);
-              pair_umma(acc, dah, dbh, idesc, 1);
+              ns_umma<true>(on, acc, dal, dbh, idesc, k > 0 || ks > 0);
+              ns_umma<true>(on, acc, dah, dbl, idesc, 1);
+              ns_umma<true>(on, acc, dah, dbh, idesc, 1);
             } else {
-              pair_umma(acc, dah, dbh, idesc, k > 0 || ks > 0);
+              ns_umma<true>(on, acc, dah, dbh, idesc, k > 0 || ks > 0);
             }
           }
-          pair_commit(&cta.b->empty[s]);
+          ns_commit<true>(on, &cta.b->empty[s]);
           last_bar = &cta.b->empty[s];
           last_par = (q / kStages) & 1;
         }
         if (!ok) break;
-        pair_commit(&cta.b->t_full[b]);
+        ns_commit<true>(on, &cta.b->t_full[b]);
         last_bar = &cta.b->t_full[b];
         last_par = (i >> 1) & 1;
       }
@@ -362,7 +391,7 @@ __device__ __forceinline__ void ns_product(NsCta<PROD>& cta, const NsMaps& mp, c
       if (last_bar) mbar_wait(last_bar, last_par);  // all issued MMAs are done
     }
   } else {
-    const int kCols = tn * 4 / kEpi;  // of this warp
+    constexpr int kCols = 1024 / kEpi;  // of this warp
     const int quad = warp & 3, group = warp >> 2;
     uint8_t* slot = smem + kStages * kStage + warp * 2 * kNsSlot;
     const uint32_t bh = smem_u32(slot), bl = bh + kNsSlot;  // hi and lo block
@@ -479,6 +508,241 @@ __device__ __forceinline__ void ns_product(NsCta<PROD>& cta, const NsMaps& mp, c
   }
 }
 
+// ------------------------------------------------ matrices of at most 128 rows
+// One CTA works through a matrix: all steps in one launch, with no barrier wider
+// than the CTA between its products (cta_group::1, tiles of 128 x 128).  What bounds
+// it is latency: a product is one or a few tiles deep, so rings and finishing warps
+// are laid out for short chains.  X X^T and A A read one operand (both sides are the
+// same rows), through eight stages of 16 KiB with one MMA a product and four of 32
+// with three; a X + B X is (a I + B) X with three MMAs, so that no tile waits for
+// its part of X (with three, the 22 bits of a I + B are as good as a X apart), through
+// two stages of 64 KiB; each finishing warp takes one 32 x 32 block.
+constexpr int kSoloEpi = 16;
+constexpr int kSoloThreads = (kSoloEpi + 2) * 32;
+constexpr int kSoloRing = 8 * kNsPart;
+constexpr int kSoloSmem = kSoloRing + kSoloEpi * 2 * kNsSlot + 1024;
+struct NsSoloBarriers {
+  uint64_t full[3][8], empty[3][8];  // [ring: one operand, one or three MMAs; two operands]
+  uint64_t t_full[2], t_empty[2], c_full[kSoloEpi];
+};
+struct NsSolo {
+  NsSoloBarriers* b;
+  uint8_t* smem;
+  volatile int* abort_flag;
+  uint32_t tmem;
+  int ring[3] = {0, 0, 0};  // uses of the rings so far
+  int q = 0, i = 0;      // finishing warps: C blocks; tiles so far
+};
+
+template <int MODE>
+__device__ __forceinline__ void ns_solo_product(NsSolo& cta, const NsMaps& mp, const NsGemmParams& p,
+                                                int first, int step, int end) {
+  constexpr bool SYM = MODE == kNsGram || MODE == kNsPoly;
+  constexpr int kEpi = kSoloEpi;
+  uint8_t* const smem = cta.smem;
+  volatile int* const abort_flag = cta.abort_flag;
+  const uint32_t tmem = cta.tmem;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int nk = (p.K + 63) / 64;
+  const bool lo = !SYM || !p.one;  // three MMAs
+  const int ring = SYM ? lo : 2, kStages = SYM ? (lo ? 4 : 8) : 2;
+  const int kStage = (SYM ? (lo ? 2 : 1) : 4) * kNsPart;
+  uint64_t *const full = cta.b->full[ring], *const empty = cta.b->empty[ring];
+  if (warp == kEpi) {
+    if (lane == 0) {
+      int q = ring == 0 ? cta.ring[0] : (ring == 1 ? cta.ring[1] : cta.ring[2]);
+      bool ok = true;
+      for (int u = first; ok && u < end && !*abort_flag; u += step) {
+        const int l = u / p.per, col = u % p.per * 128;
+        for (int k = 0; k < nk; ++k, ++q) {
+          const int s = q % kStages;
+          if (q >= kStages && !mbar_wait(&empty[s], ((q / kStages) - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = smem + s * kStage;
+          mbar_expect_tx(&full[s], kStage);
+          tma_load_3d(st, mp.ah, &full[s], 64 * k, 0, l);
+          if (lo) tma_load_3d(st + kNsPart, mp.al, &full[s], 64 * k, 0, l);
+          if (!SYM) {
+            uint8_t* sb = st + 2 * kNsPart;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              tma_load_3d(sb + h * 8192, mp.bh, &full[s], col + 64 * h, 64 * k, l);
+              if (lo) tma_load_3d(sb + kNsPart + h * 8192, mp.bl, &full[s], col + 64 * h, 64 * k, l);
+            }
+          }
+        }
+      }
+      if (!ok) *abort_flag = 1;
+      // every copy lands before shared memory is used otherwise
+      for (int j = q > kStages ? q - kStages : 0; j < q; ++j)
+        mbar_wait(&full[j % kStages], (j / kStages) & 1);
+      (ring == 0 ? cta.ring[0] : (ring == 1 ? cta.ring[1] : cta.ring[2])) = q;
+    }
+  } else if (warp == kEpi + 1) {
+    {
+      const uint32_t on = elect_lane();
+      const uint32_t idesc = ns_idesc(128, 128, SYM ? 0 : 1);
+      int q = ring == 0 ? cta.ring[0] : (ring == 1 ? cta.ring[1] : cta.ring[2]);
+      int& i = cta.i;
+      uint64_t* last_bar = nullptr;
+      uint32_t last_par = 0;
+      bool ok = true;
+      for (int u = first; ok && u < end && !__any_sync(0xffffffffu, *abort_flag); u += step, ++i) {
+        const int b = i & 1;
+        if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(&cta.b->t_empty[b], ((i >> 1) - 1) & 1))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t acc = tmem + b * 128;
+        for (int k = 0; k < nk; ++k, ++q) {
+          const int s = q % kStages;
+          if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (q / kStages) & 1))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t ah = smem_u32(smem + s * kStage), bh = SYM ? ah : ah + 2 * kNsPart;
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) {
+            const uint64_t dah = kmaj_desc(ah, 128, ks);
+            const uint64_t dbh = SYM ? dah : mnmaj_desc(bh, 64, ks);
+            if (lo) {
+              const uint64_t dal = kmaj_desc(ah + kNsPart, 128, ks);
+              const uint64_t dbl = SYM ? dal : mnmaj_desc(bh + kNsPart, 64, ks);
+              ns_umma<false>(on, acc, dal, dbh, idesc, k > 0 || ks > 0);
+              ns_umma<false>(on, acc, dah, dbl, idesc, 1);
+              ns_umma<false>(on, acc, dah, dbh, idesc, 1);
+            } else {
+              ns_umma<false>(on, acc, dah, dbh, idesc, k > 0 || ks > 0);
+            }
+          }
+          ns_commit<false>(on, &empty[s]);
+          last_bar = &empty[s];
+          last_par = (q / kStages) & 1;
+        }
+        if (!ok) break;
+        ns_commit<false>(on, &cta.b->t_full[b]);
+        last_bar = &cta.b->t_full[b];
+        last_par = (i >> 1) & 1;
+      }
+      if (!ok) *abort_flag = 1;
+      if (last_bar) mbar_wait(last_bar, last_par);  // all issued MMAs are done
+      (ring == 0 ? cta.ring[0] : (ring == 1 ? cta.ring[1] : cta.ring[2])) = q;
+    }
+  } else {
+    constexpr int kCols = 32;  // of this warp
+    const int quad = warp & 3, group = warp >> 2;
+    uint8_t* slot = smem + kSoloRing + warp * 2 * kNsSlot;
+    const uint32_t bh = smem_u32(slot), bl = bh + kNsSlot;  // hi and lo block
+    constexpr bool HAS_C = MODE == kNsPoly;
+    constexpr float kDown = 1.f / kNsScale;
+    const float al = (MODE == kNsPoly ? p.alpha : 1.f) * kDown;
+    bool stores = false;  // bulk stores issued (lane 0)
+    int& cq = cta.q;        // C blocks so far
+    int& i = cta.i;
+    auto fetch_c = [&](int c, int r, int l) {
+      if (lane == 0) {
+        if (stores) bulk_wait_read_all();  // the blocks' last contents have left
+        mbar_expect_tx(&cta.b->c_full[warp], 2 * kNsSlot);
+        tma_load_3d(slot, mp.ch, &cta.b->c_full[warp], c, r, l);
+        tma_load_3d(slot + kNsSlot, mp.cl, &cta.b->c_full[warp], c, r, l);
+      }
+    };
+    for (int u = first; u < end; u += step, ++i) {
+      const int b = i & 1;
+      const NsTile t{u / p.per, 0, u % p.per};
+      const int r0 = quad * 32;
+      const int col0 = t.tj * 128 + group * kCols;
+      const int rows = min(32, p.M - r0);  // of this warp
+      const bool work = rows > 0 && col0 < p.cols;
+      // C does not depend on the products: its first block is on the way while
+      // they finish
+      if (HAS_C && work) fetch_c(col0, r0, t.l);
+      const bool got =
+          __all_sync(0xffffffffu, *abort_flag == 0 && mbar_wait(&cta.b->t_full[b], (i >> 1) & 1));
+      if (!got) {
+        *abort_flag = 1;
+        if (HAS_C && work) mbar_wait(&cta.b->c_full[warp], cq & 1);  // the copies land first
+        break;
+      }
+      tc_fence_after();
+#pragma unroll 1
+      for (int cc = 0; cc < kCols / 32; ++cc) {
+        const int c0 = col0 + 32 * cc;
+        if (!work || c0 >= p.cols) break;  // the same for the whole warp
+        float v[32];
+        tmem_ld32(tmem + ((quad * 32) << 16) + b * 128 + group * kCols + 32 * cc, v);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] *= al;
+        if (HAS_C) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&cta.b->c_full[warp], cq & 1))) {
+            *abort_flag = 1;
+            break;
+          }
+          ++cq;
+          ns_add(bh, p.beta, v);
+          ns_add(bl, p.beta, v);
+          if (r0 == c0) {  // + a I
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] += e == lane ? p.diag : 0.f;
+          }
+        } else {
+          if (lane == 0 && stores) bulk_wait_read_all();
+          __syncwarp();
+        }
+        uint32_t w[16];
+        if (MODE == kNsLast) {
+          if (p.tall) {
+            __nv_bfloat16* o = p.out + (size_t(t.l) * p.cols + c0) * p.M + r0 + lane;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (lane < rows && c0 + e < p.cols)
+                o[size_t(e) * p.M] = __float2bfloat16_rn(v[e] * kDown);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w[e] = pack_bf16(v[2 * e] * kDown, v[2 * e + 1] * kDown);
+            ns_put(bh, w);
+            __syncwarp();
+            ns_store(bh, p.out + (size_t(t.l) * p.M + r0) * p.cols + c0, p.cols, rows, p.cols - c0,
+                     p.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0);
+          }
+          fence_async_smem();  // the next C block overwrites what was read here
+          __syncwarp();
+        } else {
+          // hi parts, then what they leave as lo parts
+          ns_split_row(v, w);
+          ns_put(bh, w);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = pack_half2(v[2 * e], v[2 * e + 1]);
+          ns_put(bl, w);
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d(mp.dh, slot, c0, r0, t.l);
+            tma_store_3d(mp.dl, slot + kNsSlot, c0, r0, t.l);
+            bulk_commit();
+            stores = true;
+          }
+        }
+        if (HAS_C && cc + 1 < kCols / 32 && c0 + 32 < p.cols) fetch_c(c0 + 32, r0, t.l);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&cta.b->t_empty[b]);
+    }
+    if (lane == 0 && stores) bulk_wait_all();
+  }
+}
+
+__device__ __forceinline__ void ns_solo_between() {
+  asm volatile("fence.proxy.async;" ::: "memory");
+  __syncthreads();
+  asm volatile("fence.proxy.async;" ::: "memory");
+}
+
 // Shared memory, barriers and TMEM of a CTA of a pair; all threads of both CTAs.
 template <int PROD>
 __device__ __forceinline__ NsCta<PROD> ns_open(uint8_t* smem_raw, NsBarriers<PROD>* b, uint32_t* tmem_base,
@@ -548,68 +812,86 @@ __global__ void __launch_bounds__(ns_threads<PROD>(), 1)
   ns_close(c.tmem);
 }
 
-// Matrices of one tile row (M <= 256): every product of a matrix belongs to one CTA
-// pair, which runs all steps of its matrices in one launch.  The pair's barrier and
-// proxy fences stand between a product's stores and the next one's loads.
 struct NsAllMaps {  // [part: hi, lo], X twice
   CUtensorMap xa[2][2], xk[2][2], xe[2][2], aa[2], ae[2], ba[2], be[2];
 };
-__device__ __forceinline__ void ns_between() {
-  // the storing threads have waited for their copies; the barrier's release and
-  // acquire order them before the peer's work, the fences across the proxies
-  asm volatile("fence.proxy.async;" ::: "memory");
-  __syncwarp();
-  cluster_sync_all();
-  asm volatile("fence.proxy.async;" ::: "memory");
-}
 
-__global__ void __launch_bounds__(ns_threads<4>(), 1)
-    ns_small_kernel(const __grid_constant__ NsAllMaps w, NsGemmParams p, int N, int steps, float a,
-                    float b, float c2) {
+__global__ void __launch_bounds__(kSoloThreads, 1)
+    ns_solo_kernel(const __grid_constant__ NsAllMaps w, NsGemmParams p, int N, int steps, float a,
+                   float b, float c) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) NsBarriers<4> bars;
+  __shared__ __align__(8) NsSoloBarriers bars;
   __shared__ uint32_t tmem_base;
   __shared__ int s_abort;
-  if (threadIdx.x < int(sizeof(NsAllMaps) / sizeof(CUtensorMap)))
-    prefetch_tmap(reinterpret_cast<const CUtensorMap*>(&w) + threadIdx.x);
-  NsCta<4> c = ns_open<4>(smem_raw, &bars, &tmem_base, &s_abort);
+  const int tid = threadIdx.x;
+  if (tid < int(sizeof(NsAllMaps) / sizeof(CUtensorMap)))
+    prefetch_tmap(reinterpret_cast<const CUtensorMap*>(&w) + tid);
+  if (tid == 0) {
+    for (int r = 0; r < 3; ++r)
+      for (int i = 0; i < 8; ++i) {
+        mbar_init(&bars.full[r][i], 1);
+        mbar_init(&bars.empty[r][i], 1);
+      }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.t_full[i], 1);
+      mbar_init(&bars.t_empty[i], kSoloEpi);
+    }
+    for (int i = 0; i < kSoloEpi; ++i) mbar_init(&bars.c_full[i], 1);
+    s_abort = 0;
+    mbar_fence_init();
+  }
+  if (tid < 32) {
+    tmem_alloc(&tmem_base, 256);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
   pdl_wait();
   pdl_trigger();
-  const int tiles = (N + kNsTile - 1) / kNsTile;
-  p.tiles_m = 1;
-  for (int l = blockIdx.x >> 1; l < p.L; l += gridDim.x >> 1) {
+  NsSolo cta;
+  cta.b = &bars;
+  cta.smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  cta.abort_flag = &s_abort;
+  cta.tmem = tmem_base;
+  const int tiles = (N + 127) / 128;
+  const bool all = ns_tiny(p.M, N);
+  p.diag = a * kNsScale;
+  for (int l = blockIdx.x; l < p.L; l += gridDim.x) {
     for (int step = 0; step < steps; ++step) {
       const int i = step & 1, last = step == steps - 1;
-      const bool all = (long long)p.M * N < kNsTinyEntries, full = all || ns_full_step(step, steps);
+      const bool three = all || ns_full_step(step, steps);
       p.per = 1;
       p.cols = p.M;
       p.K = N;
       p.one = !all;
-      const NsMaps gram{&w.xa[i][0], &w.xa[i][1], &w.xa[i][0], &w.xa[i][1],
-                        nullptr,     nullptr,     &w.ae[0],    &w.ae[1]};
-      ns_product<4, kNsGram>(c, gram, p, l, 1, l + 1);
-      ns_between();
+      const NsMaps gram{&w.xa[i][0], &w.xa[i][1], nullptr, nullptr, nullptr, nullptr, &w.ae[0], &w.ae[1]};
+      ns_solo_product<kNsGram>(cta, gram, p, l, 1, l + 1);
+      ns_solo_between();
       p.K = p.M;
-      p.one = !full;
-      p.alpha = c2;
+      p.alpha = c;
       p.beta = b;
-      const NsMaps poly{&w.aa[0], &w.aa[1], &w.aa[0], &w.aa[1],
-                        &w.ae[0], &w.ae[1], &w.be[0], &w.be[1]};
-      ns_product<4, kNsPoly>(c, poly, p, l, 1, l + 1);
-      ns_between();
+      p.one = !three;
+      const NsMaps poly{&w.aa[0], &w.aa[1], nullptr, nullptr, &w.ae[0], &w.ae[1], &w.be[0], &w.be[1]};
+      ns_solo_product<kNsPoly>(cta, poly, p, l, 1, l + 1);
+      ns_solo_between();
       p.per = tiles;
       p.cols = N;
-      p.beta = a;
       const NsMaps next{&w.ba[0],    &w.ba[1],    &w.xk[i][0],     &w.xk[i][1],
                         &w.xe[i][0], &w.xe[i][1], &w.xe[1 - i][0], &w.xe[1 - i][1]};
       if (last)
-        ns_product<4, kNsLast>(c, next, p, l * tiles, 1, (l + 1) * tiles);
+        ns_solo_product<kNsLast>(cta, next, p, l * tiles, 1, (l + 1) * tiles);
       else
-        ns_product<4, kNsStep>(c, next, p, l * tiles, 1, (l + 1) * tiles);
-      ns_between();
+        ns_solo_product<kNsStep>(cta, next, p, l * tiles, 1, (l + 1) * tiles);
+      ns_solo_between();
     }
   }
-  ns_close(c.tmem);
+  tc_fence_before();
+  __syncthreads();
+  if (tid < 32) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 256);
+  }
 }
 
 // Partial sums of squares: 8 entries at a time in fp32, the sums of those in 64
@@ -907,13 +1189,12 @@ int cyfa_newton_schulz(const void* g, int dtype, int L, int m, int n, int steps,
   q.M = w.M;
   q.out = o;
   q.tall = tall;
-  // matrices of one tile row and a few columns' tiles: one launch for all steps
-  const int tiles_n = (w.N + kNsTile - 1) / kNsTile;
-  if (w.M <= kNsTile && (tiles_n <= kNsSmallTiles || L >= 74)) {
-    set_smem(ns_small_kernel, ns_smem<4>());
-    CYFA_LAUNCH("ns_small", s,
-                (launch_cluster_k(ns_small_kernel, 2 * unsigned(std::min(L, 74)), ns_threads<4>(), 2,
-                                  ns_smem<4>(), s, t, q, w.N, steps, a, b, c)));
+  // Matrices of up to 128 rows: one CTA for all steps of a matrix, unless they are few
+  // and so wide that spreading their columns' tiles over the SMs pays for the launches.
+  if (w.M <= 128 && (w.N <= kNsSoloWidth || L >= 148 || ns_tiny(w.M, w.N))) {
+    set_smem(ns_solo_kernel, kSoloSmem);
+    CYFA_LAUNCH("ns_solo", s, (launch_k(ns_solo_kernel, unsigned(std::min(L, 148)), kSoloThreads,
+                                        kSoloSmem, s, t, q, w.N, steps, a, b, c)));
     return launch_status();
   }
   for (int step = 0; step < steps; ++step) {

@@ -45,7 +45,7 @@ def _check(g, **kw):
 
 @pytest.mark.parametrize("dtype", [BF, F])
 @pytest.mark.parametrize("shape", [(1, 1), (1, 7), (9, 1), (3, 5, 5), (2, 64, 64), (127, 509), (509, 127),
-                                   (4, 128, 256), (2, 129, 257), (300, 130), (2, 3, 40, 24), (1024, 1024), (80, 100, 1500), (3, 256, 1024), (2, 257, 300), (150, 17, 33), (2, 90, 1025),
+                                   (4, 128, 256), (2, 129, 257), (300, 130), (2, 3, 40, 24), (1024, 1024), (80, 100, 1500), (3, 256, 1024), (2, 257, 300), (150, 17, 33), (2, 90, 1025), (1, 5000), (3, 2500, 20), (128, 128), (2, 128, 129), (100, 2049),
                                    (2, 1408, 512), (512, 1408), (700, 2049)])
 def test_sizes(dtype, shape):
     _check(torch.randn(shape, generator=_gen(1), device="cuda").to(dtype))
