@@ -202,22 +202,32 @@ __device__ __forceinline__ void ns_split_row(float (&v)[32], uint32_t (&w)[16]) 
 // ------------------------------------------------ CTA pair (cta_group::2)
 // Tile load into this CTA's shared memory, completion signalled on the barrier
 // at the cluster address `bar` (the leader's).
-__device__ __forceinline__ void pair_load_3d(void* dst, const void* tmap, uint32_t bar, int x, int y,
-                                             int z) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(tmap), "r"(bar), "r"(x), "r"(y), "r"(z)
-      : "memory");
-}
-// The MMA warp runs converged, all its addresses warp-uniform, and one lane issues:
+// The load and MMA warps run converged, all addresses warp-uniform, and one lane issues:
 // with a single lane inside a divergent branch each operand was moved to the uniform
 // registers for every instruction, 1400 cycles for a 64-column block whose MMAs take
-// 512 (one) or 1536 (three).
+// 512 (one) or 1536 (three), and 500 cycles for a load.
 __device__ __forceinline__ uint32_t elect_lane() {
   uint32_t e;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
   return e;
+}
+template <bool PAIR>
+__device__ __forceinline__ void ns_load(uint32_t lane_on, void* dst, const void* tmap, uint32_t bar, int x,
+                                        int y, int z) {
+  if (PAIR)
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %6, 0;\n"
+        " @q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];\n}\n" ::"r"(smem_u32(dst)),
+        "l"(tmap), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(lane_on)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %6, 0;\n"
+        " @q cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];\n}\n" ::"r"(smem_u32(dst)),
+        "l"(tmap), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(lane_on)
+        : "memory");
 }
 template <bool PAIR>
 __device__ __forceinline__ void ns_umma(uint32_t lane_on, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
@@ -302,32 +312,33 @@ __device__ __forceinline__ void ns_product(NsCta<PROD>& cta, const NsMaps& mp, c
   const int nk = (p.K + 63) / 64;
   constexpr bool lo = PROD == 3;
   if (warp == kEpi) {
-    if (lane == 0) {
+    {
+      const uint32_t on = elect_lane();
       int& q = cta.q;
       bool ok = true;
-      for (int u = first; ok && u < end && !*abort_flag; u += step) {
+      for (int u = first; ok && u < end && !__any_sync(0xffffffffu, *abort_flag); u += step) {
         const NsTile t = ns_tile<SYM>(p, u);
         const int ra = t.ti * kNsTile + rank * 128, cb = t.tj * kNsTile + rank * 128;
         for (int k = 0; k < nk; ++k, ++q) {
           const int s = q % kStages;
-          if (q >= kStages && !mbar_wait(&cta.b->empty[s], ((q / kStages) - 1) & 1)) {
+          if (q >= kStages && !__all_sync(0xffffffffu, mbar_wait(&cta.b->empty[s], ((q / kStages) - 1) & 1))) {
             ok = false;
             break;
           }
           uint8_t* st = smem + s * kStage;
           const uint32_t bar = cluster_map(smem_u32(&cta.b->full[s]), 0);
-          if (rank == 0) mbar_expect_tx(&cta.b->full[s], 2 * kStage);  // both CTAs' bytes
-          pair_load_3d(st, mp.ah, bar, 64 * k, ra, t.l);
-          if (lo) pair_load_3d(st + kNsPart, mp.al, bar, 64 * k, ra, t.l);
+          if (rank == 0 && on) mbar_expect_tx(&cta.b->full[s], 2 * kStage);  // both CTAs' bytes
+          ns_load<true>(on, st, mp.ah, bar, 64 * k, ra, t.l);
+          if (lo) ns_load<true>(on, st + kNsPart, mp.al, bar, 64 * k, ra, t.l);
           if (SYM) {
-            pair_load_3d(st + kB, mp.bh, bar, 64 * k, cb, t.l);
-            if (lo) pair_load_3d(st + kB + kNsPart, mp.bl, bar, 64 * k, cb, t.l);
+            ns_load<true>(on, st + kB, mp.bh, bar, 64 * k, cb, t.l);
+            if (lo) ns_load<true>(on, st + kB + kNsPart, mp.bl, bar, 64 * k, cb, t.l);
           } else {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              pair_load_3d(st + kB + c * 8192, mp.bh, bar, cb + 64 * c, 64 * k, t.l);
+              ns_load<true>(on, st + kB + c * 8192, mp.bh, bar, cb + 64 * c, 64 * k, t.l);
               if (lo)
-                pair_load_3d(st + kB + kNsPart + c * 8192, mp.bl, bar, cb + 64 * c, 64 * k, t.l);
+                ns_load<true>(on, st + kB + kNsPart + c * 8192, mp.bl, bar, cb + 64 * c, 64 * k, t.l);
             }
           }
         }
@@ -549,27 +560,29 @@ __device__ __forceinline__ void ns_solo_product(NsSolo& cta, const NsMaps& mp, c
   const int kStage = (SYM ? (lo ? 2 : 1) : 4) * kNsPart;
   uint64_t *const full = cta.b->full[ring], *const empty = cta.b->empty[ring];
   if (warp == kEpi) {
-    if (lane == 0) {
+    {
+      const uint32_t on = elect_lane();
       int q = ring == 0 ? cta.ring[0] : (ring == 1 ? cta.ring[1] : cta.ring[2]);
       bool ok = true;
-      for (int u = first; ok && u < end && !*abort_flag; u += step) {
+      for (int u = first; ok && u < end && !__any_sync(0xffffffffu, *abort_flag); u += step) {
         const int l = u / p.per, col = u % p.per * 128;
         for (int k = 0; k < nk; ++k, ++q) {
           const int s = q % kStages;
-          if (q >= kStages && !mbar_wait(&empty[s], ((q / kStages) - 1) & 1)) {
+          if (q >= kStages && !__all_sync(0xffffffffu, mbar_wait(&empty[s], ((q / kStages) - 1) & 1))) {
             ok = false;
             break;
           }
           uint8_t* st = smem + s * kStage;
-          mbar_expect_tx(&full[s], kStage);
-          tma_load_3d(st, mp.ah, &full[s], 64 * k, 0, l);
-          if (lo) tma_load_3d(st + kNsPart, mp.al, &full[s], 64 * k, 0, l);
+          const uint32_t bar = smem_u32(&full[s]);
+          if (on) mbar_expect_tx(&full[s], kStage);
+          ns_load<false>(on, st, mp.ah, bar, 64 * k, 0, l);
+          if (lo) ns_load<false>(on, st + kNsPart, mp.al, bar, 64 * k, 0, l);
           if (!SYM) {
             uint8_t* sb = st + 2 * kNsPart;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              tma_load_3d(sb + h * 8192, mp.bh, &full[s], col + 64 * h, 64 * k, l);
-              if (lo) tma_load_3d(sb + kNsPart + h * 8192, mp.bl, &full[s], col + 64 * h, 64 * k, l);
+              ns_load<false>(on, sb + h * 8192, mp.bh, bar, col + 64 * h, 64 * k, l);
+              if (lo) ns_load<false>(on, sb + kNsPart + h * 8192, mp.bl, bar, col + 64 * h, 64 * k, l);
             }
           }
         }
