@@ -107,10 +107,11 @@ __device__ __forceinline__ Pair pair_mul(Pair a, Pair b) {
   const float h = a.h * b.h;
   return Pair{h, fmaf(a.h, b.l, fmaf(a.l, b.h, fmaf(a.h, b.h, -h)))};
 }
-// x + a, rounded once
+// x + a, rounded once; an infinite sum has no error to add (its parts are NaN)
 __device__ __forceinline__ float pair_add(float x, Pair a) {
   const float s = x + a.h, b = s - x;
-  return s + (((x - (s - b)) + (a.h - b)) + a.l);
+  const float r = s + (((x - (s - b)) + (a.h - b)) + a.l);
+  return fabsf(s) == INFINITY ? s : r;
 }
 // 1 / (1 + e^-z).  e^-z = 2^k e^r with r = -z - k ln 2 in [-0.35, 0.35] (ln 2 split after
 // Cody and Waite, k ln2_hi exact) and e^r from its Taylor series, the terms up to
@@ -157,7 +158,7 @@ __device__ __forceinline__ void pair_square(float y, float& s, float& c) {
 }
 // row_sum of pairs, in 64 bits
 __device__ __forceinline__ double row_sum_pair(float s, float c, double* red) {
-  double v = double(s) + double(c);
+  double v = s == INFINITY ? double(s) : double(s) + double(c);
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   const int warps = int(blockDim.x) >> 5;

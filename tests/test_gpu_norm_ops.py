@@ -216,6 +216,41 @@ def test_zero_rows_empty_and_special_values():
     assert h[1].isnan().all() and h[0].isfinite().all() and h[2].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("D", [64, 67, 1024])
+@pytest.mark.parametrize("post, gate, scale", [(False, False, "none"), (False, True, "number"),
+                                               (True, False, "vector"), (True, True, "number")])
+def test_infinities_follow_the_formula(dtype, D, post, gate, scale):
+    """Infinite and overflowing entries give the formula's infinities, zeros and NaN
+    in fp32, and leave the other rows alone.  Tolerance: one step of x's type on x'
+    (it may round to the neighbour), and on h, which is the formula of the x' returned:
+    where x and z cancel, fp32's 2^-24 |x| is any multiple of x' and so of h."""
+    ins = _inputs((7, D), dtype, post, gate, scale)
+    inf = float("inf")
+    ins["x"][0, 3], ins["x"][1, 5] = inf, -inf
+    ins["y"][2, 4], ins["y"][3, 6] = inf, -inf
+    ins["y"][4, 1] = 3e38
+    if gate:
+        ins["gate"][5, 2], ins["gate"][5, 7], ins["gate"][2, 9] = inf, -inf, -inf
+    xn, h = residual_norm(ins["x"], ins["y"], ins["weight"], ins["post_weight"], ins["gate"],
+                          ins["scale"], EPS)
+    z = ins["y"].float()
+    if post:
+        z = z * torch.rsqrt(z.pow(2).mean(-1, keepdim=True) + EPS) * ins["post_weight"]
+    if gate:
+        z = z * torch.sigmoid(ins["gate"].float())
+    x = (ins["x"].float() + z * (1.0 if ins["scale"] is None else ins["scale"])).to(dtype)
+    f = xn.float()
+    n = (f * torch.rsqrt(f.pow(2).mean(-1, keepdim=True) + EPS) * ins["weight"]).to(dtype)
+    step = 2 * HALF[dtype] if dtype == BF else 2.0 ** -18
+    for got, ref, near in ((xn, x, 4), (h, n, 0)):
+        assert torch.equal(got.isnan(), ref.isnan())
+        keep = ~ref.isnan()
+        g, r = got.double()[keep], ref.double()[keep]
+        same = g == r
+        assert (same | ((g - r).abs() <= 1.01 * step * (r.abs() + near))).all()
+
+
 def test_offsets_past_32_bits():
     stride = 2_300_000_008
     buf = torch.empty(2 * stride + 4096, device="cuda", dtype=BF)
