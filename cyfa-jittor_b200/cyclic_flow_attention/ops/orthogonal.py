@@ -37,8 +37,8 @@ def orthogonalize(g, steps=5, coefficients=QUINTIC, eps=1e-7):
         raise ValueError(f"coefficients must be three finite numbers, got {coefficients}")
     if not 0 <= steps <= 64:
         raise ValueError(f"steps must be between 0 and 64, got {steps}")
-    if not (math.isfinite(eps) and eps > 0):
-        raise ValueError(f"eps must be positive, got {eps}")
+    if not (math.isfinite(eps) and eps >= 2.0 ** -126):
+        raise ValueError(f"eps must be a positive normal fp32 number, got {eps}")
     m, n = g.shape[-2:]
     L = math.prod(g.shape[:-2])
     if L > 65535:

@@ -31,7 +31,7 @@ import torch.distributed as dist
 
 from cyclic_flow_attention import _lib
 from cyclic_flow_attention.ops import orthogonalize
-from cyclic_flow_attention.ops.orthogonal import QUINTIC
+from cyclic_flow_attention.ops.orthogonal import MAX_SIDE, QUINTIC
 
 _ALIGN = 8  # elements: 32-byte segment starts for the vectorised kernels
 
@@ -267,6 +267,8 @@ class Muon(AdamW):
         matrices = [(n, p) for n, p in named if matrix(n, p)]
         if any(p.dim() != 2 for _, p in matrices):
             raise ValueError("Muon's matrices must be two-dimensional")
+        if any(max(p.shape) > MAX_SIDE for _, p in matrices):
+            raise ValueError(f"Muon's matrices have sides up to {MAX_SIDE}")
         chosen = {id(p) for _, p in matrices}
         others = [(n, p) for n, p in named if id(p) not in chosen]
         groups = []

@@ -306,6 +306,27 @@ def test_embedding_runs(dtype):
     _embed_check(torch.full((3000,), 4, device="cuda"), w, padding_idx=4)
 
 
+@pytest.mark.parametrize("N, V", [(131072, 90000), (131073, 90000), (200003, 300), (300000, 16777300)])
+def test_embedding_many_tokens(N, V):
+    """Both sides of the number of tokens that one cluster sorts, with runs, a
+    padding row and tokens outside the vocabulary."""
+    w = torch.randn(V, 4, generator=_gen(0), device="cuda")
+    t = torch.randint(V, (N,), generator=_gen(1), device="cuda")
+    t[N // 3: N // 2] = V - 1
+    t[::7] = 5
+    _embed_check(t, w, padding_idx=5)
+    w = w.requires_grad_()
+    bad = t.clone()
+    bad[::5], bad[1::11] = -1, V
+    d = torch.randn(N, 4, generator=_gen(2), device="cuda")
+    _lib.device_error()
+    g, = torch.autograd.grad(embed_tokens(bad, w), w, d)
+    ok = (bad >= 0) & (bad < V)
+    want, = torch.autograd.grad(embed_tokens(bad[ok], w), w, d[ok])
+    assert torch.equal(g, want)  # the dropped entries come last: the same sums
+    assert _lib.device_error() == 3
+
+
 def test_embedding_misaligned_and_strided_table():
     big = torch.randn(40, 70, generator=_gen(0), device="cuda")
     t = torch.randint(40, (500,), generator=_gen(1), device="cuda")

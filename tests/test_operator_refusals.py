@@ -145,6 +145,8 @@ def test_muon_refusals_and_groups():
         Muon([])
     with pytest.raises(ValueError, match="two-dimensional"):
         Muon([b], matrix=lambda n, p: True)
+    with pytest.raises(ValueError, match="sides"):
+        Muon([torch.zeros(1 << 17, 1, requires_grad=True)])
     opt = Muon([("x.weight", w), ("lm_head.weight", torch.zeros(4, 6, requires_grad=True)), ("y", b)])
     assert [g["names"] for g in opt.param_groups] == [["x.weight"], ["lm_head.weight", "y"]]
     (w.sum() + b.sum()).backward()
