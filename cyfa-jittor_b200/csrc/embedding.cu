@@ -79,6 +79,45 @@ __global__ void __launch_bounds__(kEmbThreads)
   }
 }
 
+// The same for long rows: a warp takes 32 emb_unroll accesses of one row, so that the
+// row, its token and the addresses cost nothing per access.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kEmbThreads)
+    embed_fwd_rows_kernel(const long long* tokens, const T* w, T* out, long long N, long long V, int D,
+                          float scale, int parts) {
+  constexpr int U = emb_unroll<VEC>();
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const long long unit = (long long)blockIdx.x * (kEmbThreads / 32) + (threadIdx.x >> 5);
+  const long long n = parts == 1 ? unit : unit / parts;
+  if (n >= N) return;
+  const int c0 = (int(unit - n * parts) * (32 * U) + lane) * VEC;
+  const long long id = __ldg(tokens + n);
+  const bool ok = id >= 0 && id < V;
+  const T* src = w + (ok ? id * D : 0);
+  T* dst = out + n * D;
+  float f[U][VEC];
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int c = c0 + k * 32 * VEC;
+    if (ok && c < D) {
+      EmbVec<T, VEC>::load(src + c, f[k]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[k][e] = 0.f;
+    }
+  }
+  if (!ok && c0 == 0) set_error(kErrBadIndex);
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int c = c0 + k * 32 * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[k][e] *= scale;
+    if (c < D) EmbVec<T, VEC>::store(dst + c, f[k]);
+  }
+}
+
 // ------------------------------------------------------------------- the sort
 // Stable radix sort of (id, position), 8 bits a pass.  A CTA takes kSortTile
 // consecutive entries, each of its warps a run of them; ranks inside a run come
@@ -451,12 +490,27 @@ __global__ void __launch_bounds__(256) embed_join_kernel(EmbSumParams p) {
   const uint32_t prev = b > 0 ? p.key[b * kPiece - 1] : 0xffffffffu;
   if (v >= p.V || next != v) return;
   if (first == v && prev == v) return;  // began earlier
-  long long lo = last + 1, hi = p.N - 1;  // last entry of the run
-  while (lo < hi) {
-    const long long mid = (lo + hi + 1) >> 1;
-    if (p.key[mid] <= v) lo = mid; else hi = mid - 1;
+  // the pieces whose first entry is of the run follow this one: the first that is not
+  // among 32 at a time, a stride apart, the stride 1 at first (most runs end there)
+  const int lane = threadIdx.x & 31;
+  const long long pieces = (p.N + kPiece - 1) / kPiece;
+  auto in_run = [&](long long q) { return q < pieces && p.key[q * kPiece] == v; };
+  long long lo = b + 1, hi = pieces;  // lo: of the run, hi: not
+  int cnt = __popc(__ballot_sync(0xffffffffu, in_run(lo + 1 + lane)));
+  if (cnt < 32) {
+    lo += cnt;
+  } else {
+    lo += 32;
+    while (hi - lo > 1) {
+      const long long step = (hi - lo + 31) / 32;
+      const long long q = lo + 1 + lane * step;
+      cnt = __popc(__ballot_sync(0xffffffffu, q < hi && in_run(q)));
+      const long long top = lo + 1 + cnt * step;
+      if (cnt) lo += 1 + (cnt - 1) * step;
+      hi = top < hi ? top : hi;
+    }
   }
-  const long long parts = lo / kPiece - b, per = (parts + 7) / 8;  // head pieces
+  const long long parts = lo - b, per = (parts + 7) / 8;  // head pieces
   const int col = (threadIdx.x & 31) * VEC, g = threadIdx.x >> 5;
   for (int c0 = blockIdx.y * 32 * VEC; c0 < p.D; c0 += gridDim.y * 32 * VEC) {
     const int c = c0 + col;
@@ -540,14 +594,28 @@ int cyfa_embed_fwd(const long long* tokens, const void* weight, int dtype, void*
   const int es = dtype == 1 ? 2 : 4;
   CYFA_REQUIRE(aligned(tokens, 8) && aligned(weight, es) && aligned(out, es), kMisaligned);
   const int vec = embed_vec(D, es, weight, out);
-  const long long n = N * (D / vec), per_cta = (vec >= 4 ? 4 : 8) * kEmbThreads;
+  const int per_row = D / vec, per_thread = vec >= 4 ? 4 : 8;
+  // Rows kernel: where a row fills half of a warp's accesses or more (16384 rows of 512
+  // bf16: 12 us against 14, 65536 of 129 f32: 18 against 28; below, 65536 of 256 bf16:
+  // 24 against 19).
+  const bool by_rows = per_row * 2 >= per_thread * 32;
+  const int parts = (per_row + per_thread * 32 - 1) / (per_thread * 32);  // warps of a row
+  const long long n = by_rows ? N * parts : N * per_row;  // warps, or accesses
+  const long long per_cta = by_rows ? kEmbThreads / 32 : per_thread * kEmbThreads;
   CYFA_REQUIRE((n + per_cta - 1) / per_cta < (1ll << 31), kBadShape);
   const unsigned grid = unsigned((n + per_cta - 1) / per_cta);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-#define CYFA_EMB(T, VEC)                                                                       \
-  CYFA_LAUNCH("embed_fwd", s,                                                                  \
-              (launch_k(embed_fwd_kernel<T, VEC>, grid, kEmbThreads, 0, s, tokens,             \
-                        static_cast<const T*>(weight), static_cast<T*>(out), N, V, D, scale)))
+#define CYFA_EMB(T, VEC)                                                                        \
+  do {                                                                                          \
+    const T* w = static_cast<const T*>(weight);                                                 \
+    T* o = static_cast<T*>(out);                                                                \
+    if (by_rows)                                                                                \
+      CYFA_LAUNCH("embed_fwd", s, (launch_k(embed_fwd_rows_kernel<T, VEC>, grid, kEmbThreads, 0, \
+                                            s, tokens, w, o, N, V, D, scale, parts)));          \
+    else                                                                                        \
+      CYFA_LAUNCH("embed_fwd", s, (launch_k(embed_fwd_kernel<T, VEC>, grid, kEmbThreads, 0, s,  \
+                                            tokens, w, o, N, V, D, scale)));                    \
+  } while (0)
   if (dtype == 1) {
     if (vec == 8) CYFA_EMB(__nv_bfloat16, 8);
     else if (vec == 4) CYFA_EMB(__nv_bfloat16, 4);
@@ -600,8 +668,10 @@ int cyfa_embed_bwd(const long long* tokens, const void* dout, int dtype, void* d
     p.clear_vecs = (long long)((nbytes - lead) / 16);
     p.edge1 = d + lead + p.clear_vecs * 16;
     p.edge1_bytes = int(nbytes - lead - p.clear_vecs * 16);
-    // up to 16 clusters clear, 64 KiB a CTA at least
-    const unsigned clear = unsigned(std::min<long long>(16, 1 + p.clear_vecs / (kCsCtas * 2 * kCsClear)));
+    // 128 KiB a clearing CTA at least, up to 128 clusters: only 16 clusters run at a
+    // time, so that few large shares leave a second round (100003 x 1001 f32, 400 MB:
+    // 109 us in 16 clusters, 86 in 32, 74 in 64, 71 in 128; 32000 x 1024 bf16 25, 22, 20, 23)
+    const unsigned clear = unsigned(std::min<long long>(128, 1 + p.clear_vecs / (kCsCtas * 4 * kCsClear)));
     const dim3 grid(kCsCtas * (1 + clear));
 #define CYFA_CS(PER)                                                                             \
   do {                                                                                           \
