@@ -11,6 +11,37 @@ _NO_GUARD = contextlib.nullcontext()
 _CODES = {torch.float32: 0, torch.bfloat16: 1}
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+    """A gradient as it is, which refuses to be differentiated."""
+
+    @staticmethod
+    def forward(ctx, g, *sources):
+        return g.view_as(g)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("this operator has no second derivative")
+
+
+def first_order(backward):
+    """For the backward of an operator without a second derivative: under
+    create_graph its gradients depend on what they were computed from, and raise
+    when they are differentiated.  (``once_differentiable`` would leave out the
+    dependence on the saved tensors without a word.)"""
+
+    def run(ctx, *grads):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        sources = [t for t in (*grads, *ctx.saved_tensors) if t is not None and t.requires_grad]
+        if not sources:
+            return out
+        return tuple(g if g is None else _NoSecondDerivative.apply(g, *sources) for g in out)
+
+    return run
+
+
 def dtype_code(name, t):
     code = _CODES.get(t.dtype)
     if code is None:

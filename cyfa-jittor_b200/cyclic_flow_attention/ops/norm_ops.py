@@ -10,12 +10,17 @@ import ctypes
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._rows import address, as_rows, dtype_code, f32, on_device, same_device
+from ._rows import address, as_rows, dtype_code, f32, first_order, on_device, same_device
 
 MAX_WIDTH = 8192
+
+
+def _dense(g, dtype):
+    if g is None or (g.dtype == dtype and g.is_contiguous()):
+        return g
+    return g.to(dtype).contiguous()
 
 
 def _args(x, y, gate, weight, post, scale_vector, scale, eps):
@@ -66,7 +71,7 @@ class ResidualNormFunction(torch.autograd.Function):
         return (h,) if xn is None else (xn, h)
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, *grads):
         t, y, w, pw, gate, sv, rstd_x, rstd_y = ctx.saved_tensors
         scale, eps, plain, has_y, dtypes = ctx.meta
@@ -74,10 +79,9 @@ class ResidualNormFunction(torch.autograd.Function):
         if dxn is None and dh is None:
             return (None,) * 8
         need = ctx.needs_input_grad
-        D, dev = t.shape[-1], t.device
+        D = t.shape[-1]
         rows = t.numel() // D
-        dxn = None if dxn is None else dxn.to(t.dtype).contiguous()
-        dh = None if dh is None else dh.to(t.dtype).contiguous()
+        dxn, dh = _dense(dxn, t.dtype), _dense(dh, t.dtype)
         full = has_y and not plain
         want_x = need[0] or (plain and has_y and need[1])
         rowwise = lambda on: t.new_empty(t.shape) if on else None
@@ -91,7 +95,7 @@ class ResidualNormFunction(torch.autograd.Function):
         if rows:
             args, _keep = _args(t, y if full else None, gate, w, pw, sv, scale, eps)
             nbytes = _lib.lib().cyfa_residual_norm_bwd_work_bytes(rows, D)
-            work = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+            work = w.new_empty(nbytes // 4)
             P = address
             with on_device(t):
                 _lib.call("cyfa_residual_norm_bwd", ctypes.byref(args), rstd_x.data_ptr(),
@@ -99,9 +103,8 @@ class ResidualNormFunction(torch.autograd.Function):
                           P(dscale), work.data_ptr(), nbytes, _lib.raw_stream())
         if plain and has_y and need[1]:
             dy = dx
-        dw, dpost, dscale = (g if g is None else g.to(d)
-                             for g, d in zip((dw, dpost, dscale), dtypes))
-        return dx if need[0] else None, dy, dw, dpost, dgate, dscale, None, None
+        return (dx if need[0] else None, dy, _dense(dw, dtypes[0]), _dense(dpost, dtypes[1]), dgate,
+                _dense(dscale, dtypes[2]), None, None)
 
 
 def residual_norm(x, y, weight, post_weight=None, gate=None, scale=None, eps=1e-6):

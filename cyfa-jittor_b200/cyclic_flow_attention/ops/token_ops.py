@@ -12,10 +12,9 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._rows import address, dtype_code, f32, on_device, row_levels, same_device
+from ._rows import address, dtype_code, f32, first_order, on_device, row_levels, same_device
 
 MAX_TOP = 32
 _INTS = (torch.int64, torch.int32)
@@ -87,7 +86,7 @@ class TokenLogProbsFunction(torch.autograd.Function):
         return logp, entropy, top_logp, top_tokens
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, dlogp, dentropy, *_):
         if dlogp is None and dentropy is None:
             return None, None, None, None
@@ -169,7 +168,7 @@ class EmbedTokensFunction(torch.autograd.Function):
         return _embed_fwd(tokens, weight.contiguous(), scale)
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, dout):
         if dout is None:
             return None, None, None, None
@@ -178,10 +177,11 @@ class EmbedTokensFunction(torch.autograd.Function):
         N = tokens.numel()
         if N == 0:
             return None, torch.zeros(V, D, device=tokens.device, dtype=dtype), None, None
-        dout = dout.to(dtype).contiguous()
+        if dout.dtype != dtype or not dout.is_contiguous():
+            dout = dout.to(dtype).contiguous()
         dw = dout.new_empty((V, D))
         nbytes = _lib.lib().cyfa_embed_bwd_work_bytes(N, D)
-        work = torch.empty(nbytes, device=tokens.device, dtype=torch.uint8)
+        work = tokens.new_empty((nbytes + 7) // 8)
         with on_device(dout):
             _lib.call("cyfa_embed_bwd", tokens.data_ptr(), dout.data_ptr(),
                       dtype_code("weight", dw), dw.data_ptr(), N, V, D, scale, padding_idx,

@@ -212,3 +212,24 @@ def test_whole_training_step():
         opt.step()
     for n, p in m.named_parameters():
         assert torch.isfinite(p).all() and not torch.equal(p.detach(), before[n]), n
+
+
+def test_second_derivatives_are_refused():
+    """A gradient taken with create_graph has the ordinary values; differentiating it
+    again is an error, not a silent zero."""
+    from cyclic_flow_attention.ops import embed_tokens, residual_norm, token_log_probs
+
+    x = torch.randn(6, 32, device="cuda", requires_grad=True)
+    w = torch.rand(32, device="cuda", requires_grad=True)
+    t = torch.tensor([3, 1, 3, 0, 5, 5], device="cuda")
+    for f, saved in ((lambda: residual_norm(x, x, w)[1], True),
+                     (lambda: token_log_probs(x, t).logp, True), (lambda: embed_tokens(t, x), False)):
+        d = torch.randn_like(f())
+        plain, = torch.autograd.grad(f(), x, d)
+        for given in (d, d.clone().requires_grad_()):
+            g, = torch.autograd.grad(f(), x, given, create_graph=True)
+            assert torch.equal(g, plain)
+            for source, on in ((x, saved), (given, given.requires_grad)):
+                if on:
+                    with pytest.raises(RuntimeError, match="second derivative"):
+                        torch.autograd.grad(g.sum(), source, retain_graph=True)
