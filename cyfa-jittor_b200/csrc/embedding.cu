@@ -5,6 +5,11 @@
 // keep their order): no float atomics, the same bits on every run.  A token
 // outside the vocabulary sets the device error word, reads as a zero row and
 // has no gradient; the padding row's gradient is zero.
+// Bound by memory: the lookup of 16384 rows of 1024 bf16 takes 8 us (67 MB), 30011 of
+// 1001 f32 28 us (240 MB, the last of it left in L2).
+// The gradient of the same lookups is 62 us and 138 us: the sort beside the clearing of
+// the table (15 and 67 us; the table's 66 and 400 MB), the sums (24 and 35; 59 and
+// 200 MB) and the join of the runs that cross pieces (9 and 22, latency).
 #include <algorithm>
 #include <type_traits>
 

@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
 // matrices (cyfa_newton_schulz), over the same flat buffers:
 //   m = mu m + g,  u = g + mu m (Nesterov) or m        -> u, one dense matrix a piece
 //   master = master (1 - lr decay) - step_size o       (o: the orthogonalised u, bf16)
-// Bound by bandwidth: 16 bytes an element each.
+// Bound by bandwidth: 16 bytes an element each (momentum), 12 (apply, bf16 parameters).
 struct MuonArgs {
   BucketArgs pieces;  // momentum: ptr = u (f32); apply: ptr = the parameters
   float* m;           // momentum

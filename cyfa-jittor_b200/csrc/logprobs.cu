@@ -13,6 +13,13 @@
 // ordered(x) << 32 | ~index.  The k-th largest of the thread groups' maxima is a
 // lower bound of the k-th largest key, so a second read of the row (from cache)
 // collects the few keys above it, which are ranked by counting.
+//
+// Bound by memory where there is enough to read: 16384 rows of 32000 bf16 take 172 us
+// forward (1.05 GB at 6.1 TB/s) and 341 us backward (2.1 GB at 6.2), 93 % of what a copy
+// reaches; a thread keeps eight 16-byte loads in flight, and the entry's FMA, exponential
+// and two sums fill 60 to 70 % of the issue slots meanwhile.  One row (split over a
+// cluster) takes 9 us and 256 rows with 20 alternatives 13 us: the latency of the
+// launch, the two reads and the joins.
 #include "cyfa_common.cuh"
 
 namespace cyfa {

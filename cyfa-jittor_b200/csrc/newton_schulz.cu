@@ -18,6 +18,12 @@
 // at 1.6 times the MMAs.
 // A and B are symmetric: only the tiles on and below the diagonal are computed,
 // the others are written as their mirror images.
+//
+// Bound by the tensor cores' rate and, with one MMA a product, by shared memory and the
+// finishing warps: of five steps on 24 bf16 matrices of 2816 x 1024 (2.49 ms in all),
+// B X takes 290 us with three MMAs (425 GFLOP as issued, 1.46 PFLOP/s) and 150 with one
+// (0.95), X X^T 90 (89 GFLOP, 0.98), b A + c A A 90 and 50; splitting G into X0 92 and
+// its norms 28.  Four matrices of 127 x 509 take 113 us: 15 products one after the other.
 #include <cuda_fp16.h>
 
 #include "cyfa_common.cuh"
@@ -42,7 +48,12 @@ constexpr int kNsTile = 256;  // rows and columns of a CTA pair's tile
 __host__ __device__ constexpr bool ns_tiny(int M, int N) {
   return M < 32 || (long long)M * N < 16384;
 }
-constexpr int kNsSoloWidth = 2048;  // columns of a matrix that one CTA works through
+// Matrices of up to 128 rows: one CTA takes all steps of a matrix in one launch, if
+// they are short or many enough; otherwise their columns' tiles are spread over the SMs
+// at three launches a step (five steps, f32, with the norms and X0; one CTA a matrix
+// against spread: 4 of 128 x 512 129 us against 142, of 1024 182 against 153; of 2048:
+// 32 matrices 303 against 257, 64 334 against 358; 148 of 4096 851 against 1241).
+constexpr int kNsSoloWidth = 640, kNsSoloCount = 64;
 
 enum NsMode : int {
   kNsGram = 0,    // D = acc
@@ -1202,9 +1213,7 @@ int cyfa_newton_schulz(const void* g, int dtype, int L, int m, int n, int steps,
   q.M = w.M;
   q.out = o;
   q.tall = tall;
-  // Matrices of up to 128 rows: one CTA for all steps of a matrix, unless they are few
-  // and so wide that spreading their columns' tiles over the SMs pays for the launches.
-  if (w.M <= 128 && (w.N <= kNsSoloWidth || L >= 148 || ns_tiny(w.M, w.N))) {
+  if (w.M <= 128 && (w.N <= kNsSoloWidth || L >= kNsSoloCount || ns_tiny(w.M, w.N))) {
     set_smem(ns_solo_kernel, kSoloSmem);
     CYFA_LAUNCH("ns_solo", s, (launch_k(ns_solo_kernel, unsigned(std::min(L, 148)), kSoloThreads,
                                         kSoloSmem, s, t, q, w.N, steps, a, b, c)));
