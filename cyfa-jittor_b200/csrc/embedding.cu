@@ -7,9 +7,9 @@
 // has no gradient; the padding row's gradient is zero.
 // Bound by memory: the lookup of 16384 rows of 1024 bf16 takes 8 us (67 MB), 30011 of
 // 1001 f32 28 us (240 MB, the last of it left in L2).
-// The gradient of the same lookups is 62 us and 138 us: the sort beside the clearing of
-// the table (15 and 67 us; the table's 66 and 400 MB), the sums (24 and 35; 59 and
-// 200 MB) and the join of the runs that cross pieces (9 and 22, latency).
+// The gradient of the same lookups: the sort beside the clearing of the table (15 and
+// 66 us; the table's 66 and 400 MB), the sums (9 and 33; 59 and 200 MB) and the join of
+// the runs that cross pieces (8 and 22, latency).
 #include <algorithm>
 #include <type_traits>
 
@@ -441,13 +441,14 @@ __global__ void __launch_bounds__(kSumThreads) embed_sum_kernel(EmbSumParams p) 
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
   bool opened = key[0] == key[1];  // the current run began in an earlier piece
-  // rows in batches, a batch's loads ahead of its sums
+  // rows in batches, a batch's loads ahead of its sums; rows that do not count are read
+  // as well, since a condition at each load makes the loads wait for one another (16384
+  // tokens of 1024 bf16: 24 us against 9)
   for (int i0 = 0; i0 < cnt && key[i0 + 1] < p.V; i0 += kBatch) {
     float f[kBatch][VEC];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b)
-      if (i0 + b < cnt && key[i0 + b + 1] < p.V)
-        EmbVec<T, VEC>::load(src + (size_t)pos[i0 + b] * p.D, f[b]);
+      EmbVec<T, VEC>::load(src + (size_t)pos[min(i0 + b, cnt - 1)] * p.D, f[b]);
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int i = i0 + b;
