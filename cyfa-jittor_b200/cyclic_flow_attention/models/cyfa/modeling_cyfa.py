@@ -119,12 +119,13 @@ class CyFABlock(nn.Module):
 
 
 class CyclicFlowAttentionModel(nn.Module):
+    fused_training = False  # see CyclicFlowAttentionForCausalLM.fuse_training
+
     def __init__(self, config):
         super().__init__()
         self.embeddings = nn.Embedding(config.vocab_size, config.hidden_size)
         self.layers = nn.ModuleList([CyFABlock(config) for _ in range(config.num_hidden_layers)])
         self.norm = RMSNorm(config.hidden_size, config.norm_eps)
-        self.fused_training = False
 
     def _train_ops_ok(self, input_ids):
         w = self.embeddings.weight

@@ -100,6 +100,12 @@ def as_rows(x):
     return x, (levels[0][1] if levels else x.shape[-1])
 
 
+def dense_like(t):
+    """An uninitialised dense tensor of t's shape and type (``empty_like`` is the
+    cheaper call, but keeps other strides)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def f32(t):
     """A dense fp32 tensor with t's values (t itself when it is one)."""
     if t is None or (t.dtype == torch.float32 and t.is_contiguous()):

@@ -12,7 +12,7 @@ import math
 import torch
 
 from .. import _lib
-from ._rows import address, as_rows, dtype_code, f32, first_order, on_device, same_device
+from ._rows import address, as_rows, dense_like, dtype_code, f32, first_order, on_device, same_device
 
 MAX_WIDTH = 8192
 
@@ -42,10 +42,10 @@ def _forward(x, y, weight, post, gate, scale_vector, scale, eps, keep):
     """(xn or None, h, rstd_x, rstd_y); the last two, which only the backward
     reads, are None unless `keep`."""
     rows = x.numel() // x.shape[-1]
-    xn = None if y is None else x.new_empty(x.shape)
-    h = x.new_empty(x.shape)
+    h = dense_like(x)
+    xn = None if y is None else torch.empty_like(h)
     rstd_x = weight.new_empty(rows) if keep else None
-    rstd_y = weight.new_empty(rows) if keep and post is not None else None
+    rstd_y = torch.empty_like(rstd_x) if keep and post is not None else None
     if rows:
         args, _keep = _args(x, y, gate, weight, post, scale_vector, scale, eps)
         with on_device(x):
@@ -84,8 +84,8 @@ class ResidualNormFunction(torch.autograd.Function):
         dxn, dh = _dense(dxn, t.dtype), _dense(dh, t.dtype)
         full = has_y and not plain
         want_x = need[0] or (plain and has_y and need[1])
-        rowwise = lambda on: t.new_empty(t.shape) if on else None
-        column = lambda on: (w.new_empty(D) if rows else w.new_zeros(D)) if on else None
+        rowwise = lambda on: dense_like(t) if on else None
+        column = lambda on: (torch.empty_like(w) if rows else torch.zeros_like(w)) if on else None
         dx = rowwise(want_x)
         dy = rowwise(full and need[1])
         dgate = rowwise(gate is not None and need[4])

@@ -14,7 +14,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from .. import _lib
-from ._rows import address, dtype_code, f32, first_order, on_device, row_levels, same_device
+from ._rows import address, dense_like, dtype_code, f32, first_order, on_device, row_levels, same_device
 
 MAX_TOP = 32
 _INTS = (torch.int64, torch.int32)
@@ -92,7 +92,7 @@ class TokenLogProbsFunction(torch.autograd.Function):
             return None, None, None, None
         x, tokens, stats, entropy = ctx.saved_tensors
         x, inner, outer_stride, inner_stride = _addressed(x)
-        dx = x.new_empty(x.shape)
+        dx = dense_like(x)
         rows = tokens.numel()
         dlogp, dentropy = f32(dlogp), f32(dentropy)
         if rows:

@@ -67,6 +67,26 @@ def test_fused_step_matches_the_glue_step():
     assert rel_l2(whole[1], ref) < 1.2 * rel_l2(whole[0], ref)
 
 
+def test_fused_step_with_a_padded_batch():
+    """A right-padded batch with its attention mask, and one row without any label:
+    both paths are one bf16 computation rounded in other places, at most 40 roundings
+    of 2^-8 one after the other between a parameter's gradient and the inputs."""
+    cfg, m = _model(4)
+    ids = torch.randint(0, cfg.vocab_size, (3, 130), generator=seeded(5)).cuda()
+    mask = torch.ones_like(ids)
+    mask[0, 77:] = 0
+    labels = ids.masked_fill(mask == 0, -100)
+    labels[2] = -100
+    got = []
+    for on in (False, True):
+        m.fuse_training(on).zero_grad(set_to_none=True)
+        loss = m(ids, labels=labels, attention_mask=mask)["loss"]
+        loss.backward()
+        got.append((loss.detach(), torch.cat([p.grad.float().reshape(-1) for p in m.parameters()])))
+    assert abs(float(got[1][0]) - float(got[0][0])) < 2.0 ** -8 * abs(float(got[0][0]))
+    assert rel_l2(got[1][1], got[0][1]) < 40 * 2.0 ** -8
+
+
 def test_fused_step_captured_and_repeated():
     """The fused forward and backward in one CUDA graph, replayed: the same gradients
     as eager, bit for bit (no atomics anywhere)."""
