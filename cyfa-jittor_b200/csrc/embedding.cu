@@ -244,7 +244,9 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_move_kernel(SortPass 
 // in the CTAs' shared memory, a thread holds its own in registers while a pass
 // scatters them to their places, in whichever CTA.  A pass takes three cluster
 // barriers instead of three launches.  The grid's other clusters clear the
-// table's gradient meanwhile.
+// table's gradient meanwhile.  (The whole gradient of 64 f32 columns and 32000 rows
+// against the sort by launches above: 256 tokens 17 us against 38, 16384 28 against 66,
+// 65536 60 against 79, 131072 101 against 98; 300000 rows, 131072 tokens 122 against 134.)
 constexpr int kCsCtas = 8;
 constexpr int kCsThreads = 1024;
 constexpr int kCsWarps = kCsThreads / 32;

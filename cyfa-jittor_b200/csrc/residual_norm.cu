@@ -15,7 +15,9 @@
 // (134 MB at 6.4 TB/s) and 33 us backward (the same bytes at 4.1: a row's two reductions
 // stand between its loads and its stores); the sums of the partial rows take 3 us.
 // Rows at any alignment are bound by the issue of one access an entry: 4099 x 1531 f32
-// with both norms, gate and scale 35 us forward and 52 backward (125 and 176 MB).
+// with both norms, gate and scale 35 us forward and 52 backward (125 and 176 MB).  bf16
+// rows with a gate are bound by the arithmetic of the pairs (below): 16384 x 1024 with
+// post-norm and gate 105 us forward (134 MB) and 93 backward.
 #include <algorithm>
 
 #include "cyfa_common.cuh"
@@ -23,6 +25,7 @@
 namespace cyfa {
 
 constexpr int kRnMaxWidth = 8192;  // 1024 threads
+constexpr int kRnFewRows = 4096;  // bf16 rows that are taken 8 columns a thread
 
 struct ResNormParams {
   const void *x, *y, *gate;          // [rows, D], strides below; y and gate may be null
@@ -692,11 +695,18 @@ __global__ void __launch_bounds__(1024)
   if (threadIdx.x == 0 && cc < D) out[cc] = v;
 }
 
-// Columns of a thread: 8; with 16-byte accesses 32 once 8 would be more than a warp a
-// row (8192 columns are 256 threads), and 16 with y's side up to 4096 columns, for
-// the three accumulators a column.
-static int rn_elems(int D, bool vector, bool full) {
-  return !vector || D <= 256 ? 8 : (full && D <= 4096 ? 16 : 32);
+// Columns of a thread: 8, which leaves the most room for rows in flight, unless bf16 rows
+// are many enough that 32, a row of 1024 to a warp, saves more in barriers, or a row
+// would not fit 256 threads; with y's side 16 for the three accumulators a column.
+// Backward times in us: bf16 rows of 1024, plain, 4096 of them 20 with 8 and 23 with 32,
+// 16384 of them 46 and 42, with post-norm and gate 114 and 97; 4096 x 4096 with both 113
+// with 16, 120 with 32; f32 8192 x 2048 with both 114 with 8, 139 with 16, 4096 x 4096
+// plain 62 with 16, 66 with 32.
+static int rn_elems(int D, int es, long long rows, bool vector, bool full) {
+  if (!vector || D <= 256) return 8;
+  if (es == 4) return D <= 2048 ? 8 : (D <= 4096 ? 16 : 32);
+  if (D <= 2048 && rows <= kRnFewRows) return 8;
+  return full && D > 1024 && D <= 4096 ? 16 : 32;
 }
 // threads of a row with E columns each, and rows of a CTA
 static dim3 rn_block(int D, int E, bool vector, long long rows) {
@@ -730,7 +740,7 @@ struct RnBwdShape {
   size_t smem;
   unsigned grid;
   RnBwdShape(int D, int es, long long rows, bool full, bool gate, bool vector) {
-    elems = rn_elems(D, vector, full);
+    elems = rn_elems(D, es, rows, vector, full);
     block = rn_block(D, elems, vector, rows);
     const size_t slot = rn_slot_bytes(block, elems, es, full ? 4 + gate : 3);
     stages = rn_stages(slot);
@@ -792,7 +802,7 @@ int cyfa_residual_norm_fwd(const cyfa_residual_norm_args* a, void* xn, void* h, 
   const bool vector = rn_vector(a->D, es, {a->x, a->y, a->gate, xn, h},
                                 {a->weight, a->post_weight, a->scale_vector},
                                 {a->x_stride, a->y ? a->y_stride : 0, a->gate ? a->gate_stride : 0});
-  const int elems = rn_elems(a->D, vector, false);
+  const int elems = rn_elems(a->D, es, a->rows, vector, false);
   const dim3 block = rn_block(a->D, elems, vector, a->rows);
   const long long ctas = (a->rows + block.y - 1) / block.y;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -813,7 +823,9 @@ int cyfa_residual_norm_fwd(const cyfa_residual_norm_args* a, void* xn, void* h, 
     if (a->dtype == 1) {
       if (elems == 8) CYFA_RN(__nv_bfloat16, 8); else CYFA_RN(__nv_bfloat16, 32);
     } else {
-      if (elems == 8) CYFA_RN(float, 8); else CYFA_RN(float, 32);
+      if (elems == 8) CYFA_RN(float, 8);
+      else if (elems == 16) CYFA_RN(float, 16);
+      else CYFA_RN(float, 32);
     }
 #undef CYFA_RN
 #undef CYFA_RN_L
