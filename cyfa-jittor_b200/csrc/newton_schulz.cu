@@ -7,23 +7,19 @@
 // The products run on tcgen05 (CTA pairs) with fp32 accumulators in TMEM.  X, A
 // and B are kept as fp16 pairs hi + lo (22 significant bits), stored times 2^12:
 // that keeps the lo parts of small entries above fp16's underflow and leaves room
-// up to |entry| < 16.  A product is the three MMAs hi hi + hi lo + lo hi where its
-// rounding would show, one MMA hi hi where it does not: a X + B X cancels to a
-// tenth of its terms once the singular values are near 1, so A A and B X take all
-// three except in the first two steps (while most of them are small); A = X X^T,
-// whose error is not cancelled against anything, takes one.  Simulated
-// in 64 bits on Gaussian, low-rank and graded matrices this is within 1.5e-4 to
-// 6e-4 relative of the exact iteration, a third of the bf16 rounding of the
-// result (1.7e-3); one MMA everywhere is up to 2.8e-3 off, three everywhere 8e-7,
-// at 1.6 times the MMAs.
+// up to |entry| < 16.  Every product is the three MMAs hi hi + hi lo + lo hi: lo lo is
+// 2^-22 of it.  (hi hi alone, in X X^T and in the first steps, where fewer terms cancel,
+// took 2.5 ms in place of 3.5 for 24 matrices of 2816 x 1024, but left 6e-4 after five
+// steps, a third of the result's rounding, and more than that rounding after 16: the
+// quintic's fixed value repels, so that long runs enlarge what is lost.)
 // A and B are symmetric: only the tiles on and below the diagonal are computed,
 // the others are written as their mirror images.
 //
-// Bound by the tensor cores' rate and, with one MMA a product, by shared memory and the
-// finishing warps: of five steps on 24 bf16 matrices of 2816 x 1024 (2.49 ms in all),
-// B X takes 290 us with three MMAs (425 GFLOP as issued, 1.46 PFLOP/s) and 150 with one
-// (0.95), X X^T 90 (89 GFLOP, 0.98), b A + c A A 90 and 50; splitting G into X0 92 and
-// its norms 28.  Four matrices of 127 x 509 take 113 us: 15 products one after the other.
+// Bound by the tensor cores' rate: of five steps on 24 bf16 matrices of 2816 x 1024
+// (3.5 ms in all), B X takes 300 us a step (425 GFLOP as issued, 1.42 PFLOP/s), X X^T 219
+// (266 GFLOP, 1.22: its 240 tiles are four rounds of 74 CTA pairs, the last a quarter
+// full), b A + c A A 92; splitting G into X0 100 and its norms 31.  Four matrices of
+// 127 x 509 take 116 us: 15 products one after the other.
 #include <cuda_fp16.h>
 
 #include "cyfa_common.cuh"
@@ -31,29 +27,16 @@
 namespace cyfa {
 
 constexpr float kNsScale = 4096.f;  // 2^12
-template <int PROD>
-constexpr int ns_epi_warps() {
-  return PROD == 3 ? 8 : 16;
-}
-template <int PROD>
-constexpr int ns_threads() {
-  return (ns_epi_warps<PROD>() + 2) * 32;
-}
-// Steps whose A A and B X take three MMAs: all but the first two, and the last three.
-__host__ __device__ constexpr bool ns_full_step(int step, int steps) {
-  return step >= 2 || steps - step <= 3;
-}
+constexpr int kNsEpi = 8;            // finishing warps
+constexpr int kNsThreads = (kNsEpi + 2) * 32;
 constexpr int kNsTile = 256;  // rows and columns of a CTA pair's tile
-// Matrices whose rounding errors average over too few entries to be left at one MMA.
-__host__ __device__ constexpr bool ns_tiny(int M, int N) {
-  return M < 32 || (long long)M * N < 16384;
-}
 // Matrices of up to 128 rows: one CTA takes all steps of a matrix in one launch, if
-// they are short or many enough; otherwise their columns' tiles are spread over the SMs
-// at three launches a step (five steps, f32, with the norms and X0; one CTA a matrix
-// against spread: 4 of 128 x 512 129 us against 142, of 1024 182 against 153; of 2048:
-// 32 matrices 303 against 257, 64 334 against 358; 148 of 4096 851 against 1241).
-constexpr int kNsSoloWidth = 640, kNsSoloCount = 64;
+// they are short, low or many enough; otherwise their columns' tiles are spread over the
+// SMs at three launches a step (five steps, f32, with the norms and X0, in us; one CTA a
+// matrix against spread: 4 of 128 x 512 112 and 152, of 1024 164 and 185, 1 of 2048 268 and
+// 252, 4 of 4096 472 and 390; 32 of 4096 607 and 581, 48 of 2048 339 and 413, 64 of 4096
+// 668 and 820; 4 of 32 x 8192 565 and 639).
+constexpr int kNsSoloWidth = 1024, kNsSoloCount = 48, kNsSoloRows = 32;
 
 enum NsMode : int {
   kNsGram = 0,    // D = acc
@@ -69,26 +52,14 @@ struct NsGemmParams {
   float alpha, beta;
   __nv_bfloat16* out;       // kNsLast
   int tall;                 // out is [L, cols, M]
-  int one;                  // small matrices: one MMA a product
   float diag;               // and a in the units of D, added to B's diagonal
 };
 
-// Per stage and CTA: 128 rows of A and 128 of B, 64 contraction columns each, hi
-// and (with three products) lo.
+// Per stage and CTA: 128 rows of A and 128 of B, 64 contraction columns each, hi and lo.
 constexpr int kNsPart = 128 * 128;
 constexpr int kNsSlot = 32 * 64;  // a finishing warp's block: 32 rows x 32 columns of 16 bits
-template <int PROD>
-constexpr int ns_stage_bytes() {
-  return (PROD == 3 ? 4 : 2) * kNsPart;
-}
-template <int PROD>
-constexpr int ns_stages() {
-  return PROD == 3 ? 3 : 5;
-}
-template <int PROD>
-constexpr int ns_smem() {
-  return ns_stages<PROD>() * ns_stage_bytes<PROD>() + ns_epi_warps<PROD>() * 2 * kNsSlot + 1024;
-}
+constexpr int kNsStageBytes = 4 * kNsPart, kNsStages = 3;
+constexpr int kNsSmem = kNsStages * kNsStageBytes + kNsEpi * 2 * kNsSlot + 1024;
 
 // fp16 x fp16 -> fp32
 __host__ __device__ constexpr uint32_t ns_idesc(int M, int N, int b_mn) {
@@ -124,7 +95,7 @@ __device__ __forceinline__ NsTile ns_tile(const NsGemmParams& p, int u) {
 // the 64-byte TMA swizzle: 4 chunks of 16 bytes a row.  A lane reads and writes its
 // own row; memory is reached by TMA.  (Going to memory from the registers, by rows
 // or through a warp transposition, cost more load/store issue than the tile's
-// MMAs take: 209 us against 140 for B X on 24 matrices of 1024 x 2816.)
+// MMAs take: 209 us against 140 for B X with one MMA a product, on 24 matrices of 1024 x 2816.)
 __device__ __forceinline__ uint32_t ns_slot(uint32_t block, int row, int chunk) {
   return block + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
 }
@@ -216,7 +187,7 @@ __device__ __forceinline__ void ns_split_row(float (&v)[32], uint32_t (&w)[16]) 
 // The load and MMA warps run converged, all addresses warp-uniform, and one lane issues:
 // with a single lane inside a divergent branch each operand was moved to the uniform
 // registers for every instruction, 1400 cycles for a 64-column block whose MMAs take
-// 512 (one) or 1536 (three), and 500 cycles for a load.
+// 1536, and 500 cycles for a load.
 __device__ __forceinline__ uint32_t elect_lane() {
   uint32_t e;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
@@ -285,19 +256,16 @@ struct NsEpiMaps {
 // Persistent CTA pairs; a pair's tile is 256 x 256, CTA r of it holds rows 128 r ..
 // of the result (in its TMEM) and of A, and columns 128 r .. of B.  One warp
 // loads (one lane), one of the leader's issues the MMAs of both CTAs (one lane), the
-// EPI others finish the tile from one of the two TMEM accumulators while the next
+// kNsEpi others finish the tile from one of the two TMEM accumulators while the next
 // tile is computed into the other: warp w reads lane quadrant w & 3 (32 rows) and
-// the columns (1024 / EPI) (w >> 2) .., 32 at a time.  PROD: MMAs per
-// product (3: hi and lo parts).
-template <int PROD>
+// the columns (1024 / kNsEpi) (w >> 2) .., 32 at a time.
 struct NsBarriers {
-  uint64_t full[ns_stages<PROD>()], empty[ns_stages<PROD>()], t_full[2], t_empty[2];
-  uint64_t c_full[ns_epi_warps<PROD>()];
+  uint64_t full[kNsStages], empty[kNsStages], t_full[2], t_empty[2];
+  uint64_t c_full[kNsEpi];
 };
-// What a thread carries from one product to the next.
-template <int PROD>
+// What a thread carries through the tiles of a product.
 struct NsCta {
-  NsBarriers<PROD>* b;
+  NsBarriers* b;
   uint8_t* smem;
   volatile int* abort_flag;
   uint32_t tmem;
@@ -309,19 +277,18 @@ struct NsMaps {
 };
 
 // The tiles first, first + step, .. < end of one product.
-template <int PROD, int MODE>
-__device__ __forceinline__ void ns_product(NsCta<PROD>& cta, const NsMaps& mp, const NsGemmParams& p,
+template <int MODE>
+__device__ __forceinline__ void ns_product(NsCta& cta, const NsMaps& mp, const NsGemmParams& p,
                                            int first, int step, int end) {
   constexpr bool SYM = MODE == kNsGram || MODE == kNsPoly;
-  constexpr int kStage = ns_stage_bytes<PROD>(), kStages = ns_stages<PROD>();
-  constexpr int kEpi = ns_epi_warps<PROD>();
+  constexpr int kStage = kNsStageBytes, kStages = kNsStages;
+  constexpr int kEpi = kNsEpi;
   constexpr int kB = kStage / 2;  // B parts follow the A parts
   uint8_t* const smem = cta.smem;
   volatile int* const abort_flag = cta.abort_flag;
   const uint32_t tmem = cta.tmem;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, rank = cta.rank;
   const int nk = (p.K + 63) / 64;
-  constexpr bool lo = PROD == 3;
   if (warp == kEpi) {
     {
       const uint32_t on = elect_lane();
@@ -340,16 +307,15 @@ __device__ __forceinline__ void ns_product(NsCta<PROD>& cta, const NsMaps& mp, c
           const uint32_t bar = cluster_map(smem_u32(&cta.b->full[s]), 0);
           if (rank == 0 && on) mbar_expect_tx(&cta.b->full[s], 2 * kStage);  // both CTAs' bytes
           ns_load<true>(on, st, mp.ah, bar, 64 * k, ra, t.l);
-          if (lo) ns_load<true>(on, st + kNsPart, mp.al, bar, 64 * k, ra, t.l);
+          ns_load<true>(on, st + kNsPart, mp.al, bar, 64 * k, ra, t.l);
           if (SYM) {
             ns_load<true>(on, st + kB, mp.bh, bar, 64 * k, cb, t.l);
-            if (lo) ns_load<true>(on, st + kB + kNsPart, mp.bl, bar, 64 * k, cb, t.l);
+            ns_load<true>(on, st + kB + kNsPart, mp.bl, bar, 64 * k, cb, t.l);
           } else {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               ns_load<true>(on, st + kB + c * 8192, mp.bh, bar, cb + 64 * c, 64 * k, t.l);
-              if (lo)
-                ns_load<true>(on, st + kB + kNsPart + c * 8192, mp.bl, bar, cb + 64 * c, 64 * k, t.l);
+              ns_load<true>(on, st + kB + kNsPart + c * 8192, mp.bl, bar, cb + 64 * c, 64 * k, t.l);
             }
           }
         }
@@ -389,16 +355,12 @@ __device__ __forceinline__ void ns_product(NsCta<PROD>& cta, const NsMaps& mp, c
           for (int ks = 0; ks < 4; ++ks) {
             const uint64_t dah = kmaj_desc(ah, 128, ks);
             const uint64_t dbh = SYM ? kmaj_desc(bh, 128, ks) : mnmaj_desc(bh, 64, ks);
-            if (lo) {
-              const uint64_t dal = kmaj_desc(ah + kNsPart, 128, ks);
-              const uint64_t dbl = SYM ? kmaj_desc(bh + kNsPart, 128, ks)
-                                       : mnmaj_desc(bh + kNsPart, 64, ks);
-              ns_umma<true>(on, acc, dal, dbh, idesc, k > 0 || ks > 0);
-              ns_umma<true>(on, acc, dah, dbl, idesc, 1);
-              ns_umma<true>(on, acc, dah, dbh, idesc, 1);
-            } else {
-              ns_umma<true>(on, acc, dah, dbh, idesc, k > 0 || ks > 0);
-            }
+            const uint64_t dal = kmaj_desc(ah + kNsPart, 128, ks);
+            const uint64_t dbl = SYM ? kmaj_desc(bh + kNsPart, 128, ks)
+                                     : mnmaj_desc(bh + kNsPart, 64, ks);
+            ns_umma<true>(on, acc, dal, dbh, idesc, k > 0 || ks > 0);
+            ns_umma<true>(on, acc, dah, dbl, idesc, 1);
+            ns_umma<true>(on, acc, dah, dbh, idesc, 1);
           }
           ns_commit<true>(on, &cta.b->empty[s]);
           last_bar = &cta.b->empty[s];
@@ -535,16 +497,15 @@ __device__ __forceinline__ void ns_product(NsCta<PROD>& cta, const NsMaps& mp, c
 // than the CTA between its products (cta_group::1, tiles of 128 x 128).  What bounds
 // it is latency: a product is one or a few tiles deep, so rings and finishing warps
 // are laid out for short chains.  X X^T and A A read one operand (both sides are the
-// same rows), through eight stages of 16 KiB with one MMA a product and four of 32
-// with three; a X + B X is (a I + B) X with three MMAs, so that no tile waits for
-// its part of X (with three, the 22 bits of a I + B are as good as a X apart), through
+// same rows), through four stages of 32 KiB; a X + B X is (a I + B) X, so that no tile
+// waits for its part of X (the 22 bits of a I + B are as good as a X apart), through
 // two stages of 64 KiB; each finishing warp takes one 32 x 32 block.
 constexpr int kSoloEpi = 16;
 constexpr int kSoloThreads = (kSoloEpi + 2) * 32;
 constexpr int kSoloRing = 8 * kNsPart;
 constexpr int kSoloSmem = kSoloRing + kSoloEpi * 2 * kNsSlot + 1024;
 struct NsSoloBarriers {
-  uint64_t full[3][8], empty[3][8];  // [ring: one operand, one or three MMAs; two operands]
+  uint64_t full[2][4], empty[2][4];  // [ring: one operand, two operands]
   uint64_t t_full[2], t_empty[2], c_full[kSoloEpi];
 };
 struct NsSolo {
@@ -552,7 +513,7 @@ struct NsSolo {
   uint8_t* smem;
   volatile int* abort_flag;
   uint32_t tmem;
-  int ring[3] = {0, 0, 0};  // uses of the rings so far
+  int ring[2] = {0, 0};  // uses of the rings so far
   int q = 0, i = 0;      // finishing warps: C blocks; tiles so far
 };
 
@@ -566,14 +527,13 @@ __device__ __forceinline__ void ns_solo_product(NsSolo& cta, const NsMaps& mp, c
   const uint32_t tmem = cta.tmem;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int nk = (p.K + 63) / 64;
-  const bool lo = !SYM || !p.one;  // three MMAs
-  const int ring = SYM ? lo : 2, kStages = SYM ? (lo ? 4 : 8) : 2;
-  const int kStage = (SYM ? (lo ? 2 : 1) : 4) * kNsPart;
+  constexpr int ring = SYM ? 0 : 1, kStages = SYM ? 4 : 2;
+  constexpr int kStage = (SYM ? 2 : 4) * kNsPart;
   uint64_t *const full = cta.b->full[ring], *const empty = cta.b->empty[ring];
   if (warp == kEpi) {
     {
       const uint32_t on = elect_lane();
-      int q = ring == 0 ? cta.ring[0] : (ring == 1 ? cta.ring[1] : cta.ring[2]);
+      int& q = cta.ring[ring];
       bool ok = true;
       for (int u = first; ok && u < end && !__any_sync(0xffffffffu, *abort_flag); u += step) {
         const int l = u / p.per, col = u % p.per * 128;
@@ -587,13 +547,13 @@ __device__ __forceinline__ void ns_solo_product(NsSolo& cta, const NsMaps& mp, c
           const uint32_t bar = smem_u32(&full[s]);
           if (on) mbar_expect_tx(&full[s], kStage);
           ns_load<false>(on, st, mp.ah, bar, 64 * k, 0, l);
-          if (lo) ns_load<false>(on, st + kNsPart, mp.al, bar, 64 * k, 0, l);
+          ns_load<false>(on, st + kNsPart, mp.al, bar, 64 * k, 0, l);
           if (!SYM) {
             uint8_t* sb = st + 2 * kNsPart;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               ns_load<false>(on, sb + h * 8192, mp.bh, bar, col + 64 * h, 64 * k, l);
-              if (lo) ns_load<false>(on, sb + kNsPart + h * 8192, mp.bl, bar, col + 64 * h, 64 * k, l);
+              ns_load<false>(on, sb + kNsPart + h * 8192, mp.bl, bar, col + 64 * h, 64 * k, l);
             }
           }
         }
@@ -602,13 +562,12 @@ __device__ __forceinline__ void ns_solo_product(NsSolo& cta, const NsMaps& mp, c
       // every copy lands before shared memory is used otherwise
       for (int j = q > kStages ? q - kStages : 0; j < q; ++j)
         mbar_wait(&full[j % kStages], (j / kStages) & 1);
-      (ring == 0 ? cta.ring[0] : (ring == 1 ? cta.ring[1] : cta.ring[2])) = q;
     }
   } else if (warp == kEpi + 1) {
     {
       const uint32_t on = elect_lane();
       const uint32_t idesc = ns_idesc(128, 128, SYM ? 0 : 1);
-      int q = ring == 0 ? cta.ring[0] : (ring == 1 ? cta.ring[1] : cta.ring[2]);
+      int& q = cta.ring[ring];
       int& i = cta.i;
       uint64_t* last_bar = nullptr;
       uint32_t last_par = 0;
@@ -633,15 +592,11 @@ __device__ __forceinline__ void ns_solo_product(NsSolo& cta, const NsMaps& mp, c
           for (int ks = 0; ks < 4; ++ks) {
             const uint64_t dah = kmaj_desc(ah, 128, ks);
             const uint64_t dbh = SYM ? dah : mnmaj_desc(bh, 64, ks);
-            if (lo) {
-              const uint64_t dal = kmaj_desc(ah + kNsPart, 128, ks);
-              const uint64_t dbl = SYM ? dal : mnmaj_desc(bh + kNsPart, 64, ks);
-              ns_umma<false>(on, acc, dal, dbh, idesc, k > 0 || ks > 0);
-              ns_umma<false>(on, acc, dah, dbl, idesc, 1);
-              ns_umma<false>(on, acc, dah, dbh, idesc, 1);
-            } else {
-              ns_umma<false>(on, acc, dah, dbh, idesc, k > 0 || ks > 0);
-            }
+            const uint64_t dal = kmaj_desc(ah + kNsPart, 128, ks);
+            const uint64_t dbl = SYM ? dal : mnmaj_desc(bh + kNsPart, 64, ks);
+            ns_umma<false>(on, acc, dal, dbh, idesc, k > 0 || ks > 0);
+            ns_umma<false>(on, acc, dah, dbl, idesc, 1);
+            ns_umma<false>(on, acc, dah, dbh, idesc, 1);
           }
           ns_commit<false>(on, &empty[s]);
           last_bar = &empty[s];
@@ -654,7 +609,6 @@ __device__ __forceinline__ void ns_solo_product(NsSolo& cta, const NsMaps& mp, c
       }
       if (!ok) *abort_flag = 1;
       if (last_bar) mbar_wait(last_bar, last_par);  // all issued MMAs are done
-      (ring == 0 ? cta.ring[0] : (ring == 1 ? cta.ring[1] : cta.ring[2])) = q;
     }
   } else {
     constexpr int kCols = 32;  // of this warp
@@ -768,21 +722,19 @@ __device__ __forceinline__ void ns_solo_between() {
 }
 
 // Shared memory, barriers and TMEM of a CTA of a pair; all threads of both CTAs.
-template <int PROD>
-__device__ __forceinline__ NsCta<PROD> ns_open(uint8_t* smem_raw, NsBarriers<PROD>* b, uint32_t* tmem_base,
-                                               int* abort_flag) {
-  constexpr int kStages = ns_stages<PROD>(), kEpi = ns_epi_warps<PROD>();
+__device__ __forceinline__ NsCta ns_open(uint8_t* smem_raw, NsBarriers* b, uint32_t* tmem_base,
+                                         int* abort_flag) {
   const int tid = threadIdx.x;
   if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < kNsStages; ++i) {
       mbar_init(&b->full[i], 1);
       mbar_init(&b->empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&b->t_full[i], 1);
-      mbar_init(&b->t_empty[i], 2 * kEpi);
+      mbar_init(&b->t_empty[i], 2 * kNsEpi);
     }
-    for (int i = 0; i < kEpi; ++i) mbar_init(&b->c_full[i], 1);
+    for (int i = 0; i < kNsEpi; ++i) mbar_init(&b->c_full[i], 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -796,7 +748,7 @@ __device__ __forceinline__ NsCta<PROD> ns_open(uint8_t* smem_raw, NsBarriers<PRO
   __syncthreads();
   cluster_sync_all();  // the peer's barriers are ready
   tc_fence_after();
-  NsCta<PROD> c;
+  NsCta c;
   c.b = b;
   c.smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   c.abort_flag = abort_flag;
@@ -815,24 +767,24 @@ __device__ __forceinline__ void ns_close(uint32_t tmem) {
   }
 }
 
-template <int PROD, int MODE>
-__global__ void __launch_bounds__(ns_threads<PROD>(), 1)
+template <int MODE>
+__global__ void __launch_bounds__(kNsThreads, 1)
     ns_gemm_kernel(const __grid_constant__ CUtensorMap map_ah, const __grid_constant__ CUtensorMap map_al,
                    const __grid_constant__ CUtensorMap map_bh, const __grid_constant__ CUtensorMap map_bl,
                    const __grid_constant__ NsEpiMaps em, NsGemmParams p) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) NsBarriers<PROD> bars;
+  __shared__ __align__(8) NsBarriers bars;
   __shared__ uint32_t tmem_base;
   __shared__ int s_abort;
   if (threadIdx.x == 0) {
     prefetch_tmap(&map_ah);
     prefetch_tmap(&map_bh);
   }
-  NsCta<PROD> c = ns_open<PROD>(smem_raw, &bars, &tmem_base, &s_abort);
+  NsCta c = ns_open(smem_raw, &bars, &tmem_base, &s_abort);
   pdl_wait();
   pdl_trigger();
   const NsMaps m{&map_ah, &map_al, &map_bh, &map_bl, &em.ch, &em.cl, &em.dh, &em.dl};
-  ns_product<PROD, MODE>(c, m, p, blockIdx.x >> 1, gridDim.x >> 1, p.nunits);
+  ns_product<MODE>(c, m, p, blockIdx.x >> 1, gridDim.x >> 1, p.nunits);
   ns_close(c.tmem);
 }
 
@@ -851,8 +803,8 @@ __global__ void __launch_bounds__(kSoloThreads, 1)
   if (tid < int(sizeof(NsAllMaps) / sizeof(CUtensorMap)))
     prefetch_tmap(reinterpret_cast<const CUtensorMap*>(&w) + tid);
   if (tid == 0) {
-    for (int r = 0; r < 3; ++r)
-      for (int i = 0; i < 8; ++i) {
+    for (int r = 0; r < 2; ++r)
+      for (int i = 0; i < 4; ++i) {
         mbar_init(&bars.full[r][i], 1);
         mbar_init(&bars.empty[r][i], 1);
       }
@@ -879,23 +831,19 @@ __global__ void __launch_bounds__(kSoloThreads, 1)
   cta.abort_flag = &s_abort;
   cta.tmem = tmem_base;
   const int tiles = (N + 127) / 128;
-  const bool all = ns_tiny(p.M, N);
   p.diag = a * kNsScale;
   for (int l = blockIdx.x; l < p.L; l += gridDim.x) {
     for (int step = 0; step < steps; ++step) {
       const int i = step & 1, last = step == steps - 1;
-      const bool three = all || ns_full_step(step, steps);
       p.per = 1;
       p.cols = p.M;
       p.K = N;
-      p.one = !all;
       const NsMaps gram{&w.xa[i][0], &w.xa[i][1], nullptr, nullptr, nullptr, nullptr, &w.ae[0], &w.ae[1]};
       ns_solo_product<kNsGram>(cta, gram, p, l, 1, l + 1);
       ns_solo_between();
       p.K = p.M;
       p.alpha = c;
       p.beta = b;
-      p.one = !three;
       const NsMaps poly{&w.aa[0], &w.aa[1], nullptr, nullptr, &w.ae[0], &w.ae[1], &w.be[0], &w.be[1]};
       ns_solo_product<kNsPoly>(cta, poly, p, l, 1, l + 1);
       ns_solo_between();
@@ -1119,7 +1067,7 @@ static int ns_tmap(CUtensorMap* m, const __half* base, long long L, int rows, in
                         box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-template <int PROD, int MODE>
+template <int MODE>
 static void ns_launch(const CUtensorMap (&a)[2], const CUtensorMap (&b)[2], const CUtensorMap (&c)[2],
                       const CUtensorMap (&d)[2], NsGemmParams p, cudaStream_t s) {
   constexpr bool SYM = MODE == kNsGram || MODE == kNsPoly;
@@ -1127,11 +1075,10 @@ static void ns_launch(const CUtensorMap (&a)[2], const CUtensorMap (&b)[2], cons
   const int tiles_n = (p.cols + kNsTile - 1) / kNsTile;
   p.per = SYM ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * tiles_n;
   p.nunits = p.L * p.per;
-  set_smem(ns_gemm_kernel<PROD, MODE>, ns_smem<PROD>());
+  set_smem(ns_gemm_kernel<MODE>, kNsSmem);
   const unsigned grid = 2 * unsigned(std::min(p.nunits, 74));
   const NsEpiMaps em{c[0], c[1], d[0], d[1]};
-  launch_cluster_k(ns_gemm_kernel<PROD, MODE>, grid, ns_threads<PROD>(), 2, ns_smem<PROD>(), s, a[0],
-                   a[1], b[0], b[1], em, p);
+  launch_cluster_k(ns_gemm_kernel<MODE>, grid, kNsThreads, 2, kNsSmem, s, a[0], a[1], b[0], b[1], em, p);
 }
 
 }  // namespace cyfa
@@ -1213,7 +1160,7 @@ int cyfa_newton_schulz(const void* g, int dtype, int L, int m, int n, int steps,
   q.M = w.M;
   q.out = o;
   q.tall = tall;
-  if (w.M <= 128 && (w.N <= kNsSoloWidth || L >= kNsSoloCount || ns_tiny(w.M, w.N))) {
+  if (w.M <= 128 && (w.N <= kNsSoloWidth || L >= kNsSoloCount || w.M <= kNsSoloRows)) {
     set_smem(ns_solo_kernel, kSoloSmem);
     CYFA_LAUNCH("ns_solo", s, (launch_k(ns_solo_kernel, unsigned(std::min(L, 148)), kSoloThreads,
                                         kSoloSmem, s, t, q, w.N, steps, a, b, c)));
@@ -1221,26 +1168,20 @@ int cyfa_newton_schulz(const void* g, int dtype, int L, int m, int n, int steps,
   }
   for (int step = 0; step < steps; ++step) {
     const int i = step & 1, last = step == steps - 1;
-    const bool full = ns_full_step(step, steps);
     NsGemmParams p = q;
     p.cols = w.M;
     p.K = w.N;
-    CYFA_LAUNCH("ns_gram_1", s, (ns_launch<1, kNsGram>(t.xa[i], t.xa[i], t.ae, t.ae, p, s)));
+    CYFA_LAUNCH("ns_gram", s, (ns_launch<kNsGram>(t.xa[i], t.xa[i], t.ae, t.ae, p, s)));
     p.K = w.M;
     p.alpha = c;
     p.beta = b;
-    if (full)
-      CYFA_LAUNCH("ns_poly", s, (ns_launch<3, kNsPoly>(t.aa, t.aa, t.ae, t.be, p, s)));
-    else
-      CYFA_LAUNCH("ns_poly_1", s, (ns_launch<1, kNsPoly>(t.aa, t.aa, t.ae, t.be, p, s)));
+    CYFA_LAUNCH("ns_poly", s, (ns_launch<kNsPoly>(t.aa, t.aa, t.ae, t.be, p, s)));
     p.cols = w.N;
     p.beta = a;
     if (last)
-      CYFA_LAUNCH("ns_last", s, (ns_launch<3, kNsLast>(t.ba, t.xk[i], t.xe[i], t.xe[i], p, s)));
-    else if (full)
-      CYFA_LAUNCH("ns_step", s, (ns_launch<3, kNsStep>(t.ba, t.xk[i], t.xe[i], t.xe[1 - i], p, s)));
+      CYFA_LAUNCH("ns_last", s, (ns_launch<kNsLast>(t.ba, t.xk[i], t.xe[i], t.xe[i], p, s)));
     else
-      CYFA_LAUNCH("ns_step_1", s, (ns_launch<1, kNsStep>(t.ba, t.xk[i], t.xe[i], t.xe[1 - i], p, s)));
+      CYFA_LAUNCH("ns_step", s, (ns_launch<kNsStep>(t.ba, t.xk[i], t.xe[i], t.xe[1 - i], p, s)));
   }
   return launch_status();
 }

@@ -22,10 +22,12 @@ def orthogonalize(g, steps=5, coefficients=QUINTIC, eps=1e-7):
         A = X X^T  (X^T X for a tall matrix), (a, b, c) = ``coefficients``
 
     as bf16 [..., m, n].  With the default coefficients five steps bring every
-    singular value that is not tiny to between about 0.7 and 1.2.  The products
-    keep 22 bits of their operands and accumulate in fp32, so the error is the
-    final rounding's.  Other coefficients have to keep every entry of X, A and
-    b A + c A A below 16 in magnitude (beyond that the result is inf or NaN).
+    singular value that is not tiny to between about 0.7 and 1.2.  Every product
+    keeps 22 bits of its operands and accumulates in fp32, so the error is the
+    final rounding's (after ten steps or more with the default coefficients, whose
+    fixed value 0.868 repels by 1.58 a step, any rounding shows, fp32's too).
+    Other coefficients have to keep every entry of X, A and b A + c A A below 16
+    in magnitude (beyond that the result is inf or NaN).
     Not differentiable.
     """
     code = dtype_code("g", g)
