@@ -12,7 +12,7 @@ import math
 import torch
 
 from .. import _lib
-from ._rows import address, as_rows, dense_like, dtype_code, f32, first_order, on_device, same_device
+from ._rows import address, as_rows, dense_like, dtype_code, first_order, on_device, same_device
 
 MAX_WIDTH = 8192
 
@@ -21,6 +21,15 @@ def _dense(g, dtype):
     if g is None or (g.dtype == dtype and g.is_contiguous()):
         return g
     return g.to(dtype).contiguous()
+
+
+def _param(t):
+    """A [D] parameter as a dense fp32 tensor.  The conversion is autograd's own and stands
+    outside ResidualNormFunction, which then saves its inputs themselves: a copy made
+    inside would cut its gradients off from the parameter."""
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.to(torch.float32).contiguous()
 
 
 def _args(x, y, gate, weight, post, scale_vector, scale, eps):
@@ -60,21 +69,19 @@ class ResidualNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, weight, post, gate, scale_vector, scale, eps):
         ctx.set_materialize_grads(False)
-        w, pw, sv = f32(weight), f32(post), f32(scale_vector)
-        xn, h, rstd_x, rstd_y = _forward(x, y, w, pw, gate, sv, scale, eps, True)
+        xn, h, rstd_x, rstd_y = _forward(x, y, weight, post, gate, scale_vector, scale, eps, True)
         plain = post is None and gate is None and scale_vector is None and scale == 1.0
         # the plain sum needs y for no gradient
-        ctx.save_for_backward(x if xn is None else xn, None if plain else y, w, pw, gate, sv,
-                              rstd_x, rstd_y)
-        ctx.meta = (scale, eps, plain, y is not None,
-                    [None if t is None else t.dtype for t in (weight, post, scale_vector)])
+        ctx.save_for_backward(x if xn is None else xn, None if plain else y, weight, post, gate,
+                              scale_vector, rstd_x, rstd_y)
+        ctx.meta = (scale, eps, plain, y is not None)
         return (h,) if xn is None else (xn, h)
 
     @staticmethod
     @first_order
     def backward(ctx, *grads):
         t, y, w, pw, gate, sv, rstd_x, rstd_y = ctx.saved_tensors
-        scale, eps, plain, has_y, dtypes = ctx.meta
+        scale, eps, plain, has_y = ctx.meta
         dxn, dh = grads if has_y else (None, grads[0])
         if dxn is None and dh is None:
             return (None,) * 8
@@ -103,8 +110,7 @@ class ResidualNormFunction(torch.autograd.Function):
                           P(dscale), work.data_ptr(), nbytes, _lib.raw_stream())
         if plain and has_y and need[1]:
             dy = dx
-        return (dx if need[0] else None, dy, _dense(dw, dtypes[0]), _dense(dpost, dtypes[1]), dgate,
-                _dense(dscale, dtypes[2]), None, None)
+        return dx if need[0] else None, dy, dw, dpost, dgate, dscale, None, None
 
 
 def residual_norm(x, y, weight, post_weight=None, gate=None, scale=None, eps=1e-6):
@@ -144,10 +150,9 @@ def residual_norm(x, y, weight, post_weight=None, gate=None, scale=None, eps=1e-
     if not (math.isfinite(number) and math.isfinite(eps) and eps >= 0):
         raise ValueError(f"scale and eps must be finite and eps >= 0, got {scale}, {eps}")
     same_device(x, y, weight, post_weight, gate, scale_vector)
-    tensors = (x, y, weight, post_weight, gate, scale_vector)
+    tensors = (x, y, _param(weight), _param(post_weight), gate, _param(scale_vector))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         out = ResidualNormFunction.apply(*tensors, number, float(eps))
         return (x, out[0]) if y is None else out
-    xn, h, _, _ = _forward(x, y, f32(weight), f32(post_weight), gate, f32(scale_vector), number,
-                           float(eps), False)
+    xn, h, _, _ = _forward(*tensors, number, float(eps), False)
     return x if xn is None else xn, h
