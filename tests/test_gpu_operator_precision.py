@@ -41,6 +41,26 @@ def test_bf16_weight_gradient(rows, D, scale):
     assert not bad.any(), int(bad.sum())
 
 
+@pytest.mark.parametrize("D", [64, 67, 4096])
+def test_f32_gate_gradients_over_its_range(D):
+    """dy = dx' sigmoid(gate) and dgate = dx' y sigmoid (1 - sigmoid) of fp32 rows, entry by
+    entry, for gates from -86 to 86 (nothing leaves the normal range).  expf: 2 ulp = 2^-22,
+    its sum 2^-24, the reciprocal 2^-23, their product 2^-24: 2^-21, and dx' = 1 adds nothing.
+    dgate: two such factors and six products: below 2^-19.  (z < 0 and z > 0: neither 1 - sigmoid nor the
+    exponential's argument may lose bits.)"""
+    rows = 4096 // D + 8
+    gate = torch.linspace(-86, 86, rows * D, device="cuda").view(rows, D).requires_grad_()
+    y = 0.5 + torch.rand(rows, D, generator=_gen(D), device="cuda")
+    y = torch.where(torch.rand(rows, D, generator=_gen(1), device="cuda") < 0.5, -y, y).requires_grad_()
+    xn, _ = residual_norm(torch.zeros(rows, D, device="cuda"), y, torch.ones(D, device="cuda"), gate=gate)
+    dgate, dy = torch.autograd.grad(xn, (gate, y), torch.ones_like(xn))
+    z = gate.detach().double()
+    q, rest = torch.sigmoid(z), torch.sigmoid(-z)
+    assert ((dy.double() - q).abs() <= 2.0 ** -21 * q).all()
+    want = y.detach().double() * q * rest
+    assert ((dgate.double() - want).abs() <= 2.0 ** -19 * want.abs()).all()
+
+
 def _newton_schulz(g, steps, q):
     x = g.double()
     tall = x.shape[-2] > x.shape[-1]
