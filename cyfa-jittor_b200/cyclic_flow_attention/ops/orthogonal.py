@@ -15,6 +15,14 @@ QUINTIC = (3.4445, -4.7750, 2.0315)
 MAX_SIDE = 1 << 16
 
 
+def check_iteration(steps, coefficients):
+    """Raises on steps or coefficients that ``orthogonalize`` does not take."""
+    if len(coefficients) != 3 or not all(math.isfinite(c) for c in coefficients):
+        raise ValueError(f"coefficients must be three finite numbers, got {coefficients}")
+    if not 0 <= steps <= 64:
+        raise ValueError(f"steps must be between 0 and 64, got {steps}")
+
+
 def orthogonalize(g, steps=5, coefficients=QUINTIC, eps=1e-7):
     """The Newton-Schulz image of each matrix of ``g`` [..., m, n] (bf16 or fp32):
 
@@ -35,10 +43,7 @@ def orthogonalize(g, steps=5, coefficients=QUINTIC, eps=1e-7):
         raise ValueError("orthogonalize has no backward; call it under torch.no_grad()")
     if g.dim() < 2 or max(g.shape[-2:]) > MAX_SIDE:
         raise ValueError(f"g must be [..., m, n] with sides up to {MAX_SIDE}, got {tuple(g.shape)}")
-    if len(coefficients) != 3 or not all(math.isfinite(c) for c in coefficients):
-        raise ValueError(f"coefficients must be three finite numbers, got {coefficients}")
-    if not 0 <= steps <= 64:
-        raise ValueError(f"steps must be between 0 and 64, got {steps}")
+    check_iteration(steps, coefficients)
     if not (math.isfinite(eps) and eps >= 2.0 ** -126):
         raise ValueError(f"eps must be a positive normal fp32 number, got {eps}")
     m, n = g.shape[-2:]

@@ -31,7 +31,7 @@ import torch.distributed as dist
 
 from cyclic_flow_attention import _lib
 from cyclic_flow_attention.ops import orthogonalize
-from cyclic_flow_attention.ops.orthogonal import MAX_SIDE, QUINTIC
+from cyclic_flow_attention.ops.orthogonal import MAX_SIDE, QUINTIC, check_iteration
 
 _ALIGN = 8  # elements: 32-byte segment starts for the vectorised kernels
 
@@ -263,6 +263,7 @@ class Muon(AdamW):
                  eps=1e-8, adamw_weight_decay=0.01):
         if lr < 0 or weight_decay < 0 or not 0 <= momentum < 1 or steps < 1:
             raise ValueError("Invalid Muon hyperparameters")
+        check_iteration(steps, coefficients)
         named = [p if isinstance(p, tuple) else (f"0.{i}", p) for i, p in enumerate(params)]
         matrices = [(n, p) for n, p in named if matrix(n, p)]
         if any(p.dim() != 2 for _, p in matrices):
