@@ -219,7 +219,14 @@ class CyclicFlowAttentionForCausalLM(nn.Module):
 
     def fuse_training(self, on=True):
         """Runs the embedding, the residual norms and the loss of training forwards
-        (bf16 weights on a CUDA device) on the libcyfa operators; returns self."""
+        (bf16 weights on a CUDA device) on the libcyfa operators; returns self.
+
+        The adds and norms are taken out of their modules: a block's ``attn`` and
+        ``mlp`` are called as modules, but the blocks, their norms, the last norm and
+        the embedding are not, so that hooks on those, and a replaced ``forward`` of
+        theirs, do not run.  A token or label outside the vocabulary does not stop the
+        GPU as in PyTorch: the token's embedding reads as zeros, the label makes the loss
+        NaN, and the device error word becomes 3 (``_lib.device_error()``)."""
         self.model.fused_training = bool(on)
         return self
 
