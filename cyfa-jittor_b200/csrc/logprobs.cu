@@ -6,8 +6,9 @@
 //   d/dx_j (g log p_id + h H) = g [j = id] - p_j (g + h (log p_j + H))
 // One pass over the row keeps (m, s, t) per thread, all in fp32, and rescales
 // the sums when a larger maximum arrives.  Masked entries (-inf) have p = 0 and
-// add nothing; a row with no finite entry has log p = -inf, H = 0 and zero
-// gradient; NaN or +inf in a row makes its log p and H NaN.
+// add nothing; a row with no finite entry has log p = -inf, H = 0 and p = 0 throughout,
+// so that its gradient is g at id and 0 elsewhere, as at any masked id; NaN or +inf in
+// a row makes its log p and H NaN.
 //
 // Alternatives are ordered by (logit, then lowest index), as the 64-bit key
 // ordered(x) << 32 | ~index.  The k-th largest of the thread groups' maxima is a

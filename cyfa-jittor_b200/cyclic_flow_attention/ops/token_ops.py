@@ -117,8 +117,10 @@ def token_log_probs(logits, tokens, top=0, ignore_index=-100):
       tokens, by logit and among equals by lowest index; None when ``top`` is 0.
 
     Gradients flow to the logits from ``logp`` and ``entropy`` (not from the
-    alternatives), in the logits' dtype.  A masked logit (-inf) has probability 0;
-    a position with no finite logit has logp -inf, entropy 0 and zero gradient;
+    alternatives), in the logits' dtype: ``dlogp`` at the token's entry, less the
+    probabilities' share.  A masked logit (-inf) has probability 0.  A position with
+    no finite logit has logp -inf, entropy 0 and every probability 0, so that only the
+    token's entry has a gradient, ``dlogp``; with ``ignore_index`` as its token it has none.
     NaN or +inf makes the position's results NaN.  A token outside the vocabulary
     gives NaN and sets the device error word (``_lib.device_error()`` returns 3).
     """

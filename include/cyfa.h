@@ -434,7 +434,8 @@ int cyfa_swiglu(const void* gu, void* out, int rows, int mid, void* stream);
  * alignment is needed.  tokens [rows] i64: a row whose token is ignore_index has
  * logp 0 and no gradient from it; any other token outside [0, V) gives NaN, no
  * gradient and device error 3.  Masked logits (-inf) have probability 0; a row with
- * no finite logit has logp -inf, entropy 0 and zero gradient.
+ * no finite logit has logp -inf, entropy 0 and every probability 0: its gradient is
+ * dlogp at its token (none for ignore_index) and 0 elsewhere.
  * stats [rows, 2] f32 (row maximum, log of the sum) is kept for the backward (NULL without one);
  * top_logp / top_tokens [rows, top] may be NULL when top is 0. */
 int cyfa_token_logprobs_fwd(const void* logits, int dtype, long long rows, long long inner,

@@ -1,9 +1,12 @@
-"""How many bits the language-model operators keep, against 64-bit computations."""
+"""How many bits the language-model operators keep, against 64-bit computations, and
+their values where a mask leaves nothing."""
+
+import math
 
 import pytest
 import torch
 
-from cyclic_flow_attention.ops import orthogonalize, residual_norm
+from cyclic_flow_attention.ops import orthogonalize, residual_norm, token_log_probs
 
 pytestmark = pytest.mark.gpu
 BF, F = torch.bfloat16, torch.float32
@@ -108,3 +111,22 @@ def test_newton_schulz_error_is_the_final_rounding(m, n, coefficients):
             off = (orthogonalize(g, steps, coefficients).double() - ref).norm()
             plain = torch.maximum(1.02 * alone, 3 * steps * 2.0 ** -19 * ref.norm())
             assert off <= plain + grown, (steps, float(off / alone))
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("V", [1, 7, 90, 5000, 40000])
+def test_log_probs_rows_without_a_finite_logit(V, dtype):
+    """Every probability is 0, so the formula leaves dlogp at the token's entry, exactly
+    (one rounding to the logits' type), nothing from the entropy, and nothing at all where
+    the token is ignored."""
+    x = torch.full((4, V), -math.inf, device="cuda", dtype=dtype)
+    x[0] = torch.randn(V, generator=_gen(V), device="cuda").to(dtype)
+    x.requires_grad_()
+    tokens = torch.tensor([0, V - 1, -100, V // 2], device="cuda")
+    r = token_log_probs(x, tokens)
+    assert r.logp.tolist()[1:] == [-math.inf, 0, -math.inf] and (r.entropy[1:] == 0).all()
+    g, h = torch.randn(2, 4, generator=_gen(V + 1), device="cuda")
+    dx, = torch.autograd.grad((r.logp, r.entropy), x, (g, h))
+    want = torch.zeros(4, V, device="cuda", dtype=dtype)
+    want[1, V - 1], want[3, V // 2] = g[1].to(dtype), g[3].to(dtype)
+    assert torch.equal(dx[1:], want[1:]) and dx[0].isfinite().all()
