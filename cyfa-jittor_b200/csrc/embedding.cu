@@ -1,8 +1,10 @@
 // Embedding lookup with a scale, and the gradient of the whole table.
 //   out[n] = scale W[id_n]
-//   dW[v]  = scale sum over {n : id_n = v} of dout[n], in ascending n, fp32
+//   dW[v]  = scale sum over {n : id_n = v} of dout[n], fp32
 // The sum runs over the tokens sorted by id (a stable radix sort, so equal ids
-// keep their order): no float atomics, the same bits on every run.  A token
+// keep their order), in a fixed tree: up to 32 neighbours in ascending n, the partial
+// sums of a longer run in eight stretches side by side, the stretches in order.  No float
+// atomics, the same bits on every run.  A token
 // outside the vocabulary sets the device error word, reads as a zero row and
 // has no gradient; the padding row's gradient is zero.
 // Bound by memory: the lookup of 16384 rows of 1024 bf16 takes 8 us (67 MB), 30011 of

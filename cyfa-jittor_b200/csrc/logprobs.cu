@@ -18,7 +18,7 @@
 // Bound by memory where there is enough to read: 16384 rows of 32000 bf16 take 172 us
 // forward (1.05 GB at 6.1 TB/s) and 341 us backward (2.1 GB at 6.2), 93 % of what a copy
 // reaches; a thread keeps eight 16-byte loads in flight, and the entry's FMA, exponential
-// and two sums fill 60 to 70 % of the issue slots meanwhile.  One row (split over a
+// and two sums fill 74 % (forward) and 90 % (backward) of the issue slots meanwhile.  One row (split over a
 // cluster) takes 9 us and 256 rows with 20 alternatives 13 us: the latency of the
 // launch, the two reads and the joins.
 #include "cyfa_common.cuh"

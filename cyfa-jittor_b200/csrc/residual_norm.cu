@@ -8,16 +8,17 @@
 //   dgate = dt scale z sigmoid(gate) (1 - sigmoid(gate)),  dscale = sum dt sigmoid(gate) z
 //   dy    = dz    or  (dz post - y^ mean(dz post y^)) / rms(y)
 //   dweight = sum dh x^,   dpost = sum dz y^   (over the rows)
-// All arithmetic is fp32.  Each thread owns E columns of a row (kept in registers
-// between the reductions and the stores), so every tensor is read and written
-// once; column sums go through per-CTA partial rows added in a fixed order.
-// Bound by memory for 16-byte rows: 16384 x 1024 bf16, the plain sum, 21 us forward
-// (134 MB at 6.4 TB/s) and 33 us backward (the same bytes at 4.1: a row's two reductions
+// The arithmetic is fp32, but for the branch of bf16 rows ahead of x', which is carried in
+// pairs of fp32 numbers with its row sums in 64 bits (below).  Each thread owns E columns
+// of a row (kept in registers between the reductions and the stores), so every tensor is
+// read and written once; column sums go through per-CTA partial rows added in a fixed order.
+// Bound by memory for 16-byte rows: 16384 x 1024 bf16, the plain sum, 22 us forward
+// (134 MB at 6.1 TB/s) and 35 us backward (the same bytes at 3.8: a row's two reductions
 // stand between its loads and its stores); the sums of the partial rows take 3 us.
 // Rows at any alignment are bound by the issue of one access an entry: 4099 x 1531 f32
-// with both norms, gate and scale 35 us forward and 52 backward (125 and 176 MB).  bf16
+// with both norms, gate and scale 34 us forward and 55 backward (125 and 201 MB).  bf16
 // rows with a gate are bound by the arithmetic of the pairs (below): 16384 x 1024 with
-// post-norm and gate 105 us forward (134 MB) and 93 backward.
+// post-norm and gate 93 us forward (168 MB); 90 backward (268 MB), which has no pairs.
 #include <algorithm>
 
 #include "cyfa_common.cuh"
@@ -99,7 +100,8 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 // Branch arithmetic.  A bf16 stream is normalised after it is rounded, so every error
 // of x' before that rounding moves some entries to the neighbouring bf16 value, 2^-8
 // off: with plain fp32 arithmetic one entry in 2^16, which is what then limits
-// dweight's distance from the exact sum (1e-5 relative).  For bf16 rows the branch is
+// dweight's distance from the exact sum (1e-5 relative on average, 2e-4 for a few rows
+// where one entry moves; exact x': 1e-7).  For bf16 rows the branch is
 // therefore carried in pairs of fp32 numbers (value + error: 2^-29 with a gate, 2^-40
 // without), and x' is the exact sum's rounding but for one entry in 10^7 (16.7 M
 // entries: 0 or 1 off, against 220 to 560 of the plain formula).  fp32 rows use single
@@ -127,7 +129,7 @@ __device__ __forceinline__ float pair_add(float x, Pair a) {
 __device__ __forceinline__ Pair pair_sigmoid(float z) {
   const float a = fminf(fmaxf(-z, -87.f), 87.f);  // (NaN: any)
   const float k = rintf(a * 1.44269504f);
-  // ln 2 = 45426 / 65536 + 1.4285946e-6 + rest
+  // ln 2 = 45426 / 65536 + 1.4286068e-6
   const float r0 = fmaf(-k, 0.693145751953125f, a);
   const float p = k * 1.42860682e-6f;
   const float rh = r0 - p, rl = (r0 - rh) - p;

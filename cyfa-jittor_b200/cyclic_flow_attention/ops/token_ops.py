@@ -1,5 +1,5 @@
 """The two ends of the language model: ``embed_tokens`` (scaled lookup, table
-gradient summed in token order) and ``token_log_probs`` (log probability of given
+gradient summed in a fixed order) and ``token_log_probs`` (log probability of given
 tokens, entropy and most likely alternatives straight from the logits).
 
 The reference computes both with framework ops (models/cyfa/modeling_cyfa.py:58-69
@@ -197,8 +197,8 @@ def embed_tokens(tokens, weight, scale=1.0, padding_idx=None):
     ``tokens`` [...] int64 or int32 and ``weight`` [V, D] bf16 or fp32, on one CUDA
     device; the result [..., D] has the weight's dtype (one rounding after the
     fp32 product).  The gradient is the dense [V, D] table: each row sums its
-    tokens' gradient rows in fp32 in token order (the tokens are sorted, no float
-    atomics) and is rounded once; ``padding_idx`` (as in ``nn.Embedding``) gets a
+    tokens' gradient rows in fp32 in a fixed tree over the token order (the tokens are
+    sorted, no float atomics) and is rounded once; ``padding_idx`` (as in ``nn.Embedding``) gets a
     zero row.  A token outside the vocabulary reads as zeros, has no gradient and
     sets the device error word (``_lib.device_error()`` returns 3).
     """

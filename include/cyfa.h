@@ -460,8 +460,8 @@ int cyfa_embed_fwd(const long long* tokens, const void* weight, int dtype, void*
                    long long V, int D, float scale, void* stream);
 
 /* The whole table's gradient dweight [V, D] (weight's dtype, every row written):
- * row v is scale times the sum, in f32 and in ascending n, of dout[n] over the
- * tokens equal to v; the rows of tokens that do not occur and of padding_idx (-1:
+ * row v is scale times the sum of dout[n] over the tokens equal to v, in f32 and in a
+ * fixed tree over ascending n; the rows of tokens that do not occur and of padding_idx (-1:
  * none) are zero.  The tokens are sorted first, so the result does not depend on
  * the order in which CTAs run.  N < 2^31, V < 2^31.  work: 256-byte aligned. */
 size_t cyfa_embed_bwd_work_bytes(long long N, int D);
